@@ -233,6 +233,95 @@ int  oxb_hip_kv_quantize_rows(int kv_dtype, const float* rows, uint32_t n_rows, 
  * crates/oxibonsai-core/src/quant_fp8.rs), with the widening of the codes that the attention kernels use; n % 4 == 0. */
 int  oxb_hip_kv_dequantize_rows(int kv_dtype, const uint8_t* codes, const float* scales, uint32_t n_rows, uint32_t n, float* rows);
 
+/* ---- a serving step over a paged cache, on device buffers: what a server that batches requests of different lengths needs
+ * between the products (the reference's PagedKvCache does the bookkeeping on the host, write_kv and the attention one token at
+ * a time: crates/oxibonsai-model/src/paged_kv_cache.rs:375-470, layers/attention_fused.rs:329-400).  Every pointer is a DEVICE
+ * pointer that the caller owns, also the workspace; the calls launch on the stream in use, allocate nothing, wait for nothing
+ * and keep nothing, so they may be captured into a graph, which then reads whatever the buffers hold at each replay.  Lengths
+ * and page numbers live on the GPU and cannot be refused by a call: what they may name is checked by the kernels, and no value
+ * makes them leave their buffers.  The library runs on one device (oxb_hip_init): a pointer of another one is refused. */
+enum { OXB_DTYPE_F32 = 0, OXB_DTYPE_F16 = 1, OXB_DTYPE_BF16 = 2 };
+/* One layer's rows: k, v [nkv][n_pages][page_size][hd], fp16 numbers or one-byte codes (OXB_KV_DTYPE_*), 16-byte aligned; one-byte
+ * rows with their scales [nkv][n_pages][page_size] (>= 0).  This is how a model keeps the rows of a layer in a paged cache.  A
+ * slot is page * page_size + position in page, below 2^31.  page_size 16, 32, 64 or 128; hd 32, 64, 128 or 256. */
+typedef struct {
+    void *d_k, *d_v;
+    float *d_k_scale, *d_v_scale;   /* fp16 rows: not read */
+    uint32_t kv_dtype, nkv, hd, page_size, n_pages;
+} oxb_page_pool;
+/* Page tables, slot map and positions of a step from the requests' lengths.  Request r has past[r] tokens in the cache, keeps
+ * the first min(keep[r], past[r]) of them (keep NULL: all; 0: it has ended; a shared prefix' length: it has ended and the
+ * prefix' pages are not its own; past - k: k drafted tokens were rejected) and gets add[r] new ones.
+ *   1. its pages behind the kept tokens go back on top of the free ones: tables[r][ceil(kept / page_size)] .. , request by request
+ *   2. the pages that the new tokens need come from the top, free_pages[n_free - 1] first, request by request
+ *   3. cu_tokens[r + 1] = sum of add[0 .. r], cu_pages[r + 1] = sum of the pages taken, lens[r] = kept + add[r];
+ *      row cu_tokens[r] + i stands for the request's i-th new token: positions = kept + i, slots = where it lies.
+ *      Rows behind the last token have slot and position -1.
+ * All or nothing: status[0] is 0, or 1 (too few free pages), 2 (a table row or the slot map is too short), 3 (a negative length,
+ * or counts that do not fit the pool), and then tables, free pages and n_free stay, lens = past, cu_tokens and cu_pages are 0
+ * and every row is -1; status[1] = the pages that the new tokens need.  lens may be past, n_free_out may be n_free; else no
+ * two buffers overlap.  n_requests 1 .. 4096. */
+typedef struct {
+    uint32_t n_requests, page_size, n_pages, table_width, n_rows;
+    const int32_t *d_past, *d_keep, *d_add;   /* [n_requests] */
+    int32_t* d_tables;                        /* [n_requests][table_width] page numbers */
+    int32_t* d_free_pages;                    /* [n_pages], the first n_free in use */
+    const int32_t* d_n_free;
+    int32_t *d_n_free_out, *d_lens;           /* [1], [n_requests] */
+    int32_t *d_cu_tokens, *d_cu_pages;        /* [n_requests + 1] */
+    int32_t *d_slots, *d_positions;           /* [n_rows] */
+    int32_t* d_status;                        /* [2] */
+} oxb_page_assign;
+int  oxb_hip_paged_assign_dev(const oxb_page_assign* a);
+/* The step's new rows: row t of qkv holds nq q heads, nkv k heads and nkv v heads of hd values.  q and k heads go through
+ * RMSNorm with q_norm / k_norm [hd] (each may be NULL: not normed) and RoPE on the pairs (d, d + hd / 2) with the rows
+ * cos, sin [n_angles][hd / 2] of the row's position (both NULL: not rotated), as fused_qk_norm_rope does
+ * (KG/cuda_attn_kernels.rs:160-226); q goes to q_out [n_rows][nq][hd] (NULL: q is not looked at), k and v to slot slots[t] of the
+ * pool: rounded to fp16, or as codes round(x / scale) of oxb_hip_kv_quantize_rows' types with scale = max|x| times the fp32
+ * reciprocal of the largest code, at least 2^-23 (the quantiser's own scale is the quotient: an ulp apart at most).  A row whose position is negative (or has no angles, where it
+ * is rotated) is left out; one whose slot is negative or behind the pool leaves no k and v.  positions may be NULL where nothing
+ * is rotated: no row is left out then.  Two rows with one slot leave a mixture there.  Strides are in elements, multiples of 8;
+ * qkv and q_out 16-byte aligned. */
+typedef struct {
+    uint32_t n_rows, nq;
+    const void* d_qkv;
+    uint32_t qkv_dtype, qkv_stride;
+    const int32_t *d_positions, *d_slots;     /* [n_rows] */
+    const float *d_q_norm, *d_k_norm, *d_cos, *d_sin;
+    uint32_t n_angles;
+    float eps;
+    void* d_q_out;
+    uint32_t q_dtype, q_stride;
+    oxb_page_pool pool;
+} oxb_paged_rows;
+int  oxb_hip_paged_rows_dev(const oxb_paged_rows* a);
+/* Attention of a step's queries over the pool.  Request r's queries are the rows cu_tokens[r] .. cu_tokens[r + 1] - 1 of
+ * q [n_tokens][nq][hd] (nq a multiple of pool.nkv, at most 16 q heads to a kv head); the one at position p sees the keys
+ * 0 .. min(p + 1, lens[r]) - 1 of its request, key i in row i % page_size of page tables[r][i / page_size]; q head h reads
+ * kv head h / (nq / nkv):  out = sum softmax(scale * q . k) v, lse = log sum exp(scale * q . k), natural, [n_tokens][nq] or NULL.
+ * A query that sees nothing (position -1) has out 0 and lse -infinity.  Rows in front of cu_tokens[0] or behind
+ * cu_tokens[n_requests] are left as they are.
+ * Requests cu_groups[g] .. cu_groups[g + 1] - 1 share their first prefix_lens[g] keys (at most the shortest of them): those are
+ * the ones that the group's FIRST request's table names, and are read once for all the group's queries.  n_groups 0: nothing is
+ * shared; else cu_groups[0] = 0 and cu_groups[n_groups] = n_requests.
+ * q, out: one type (f32: fp32-level accuracy, scores and probabilities as two fp16 terms; f16, bf16: probabilities are
+ * rounded to fp16).  Strides in elements, multiples of 8; 16-byte aligned.  scale 0 stands for 1 / sqrt(hd).  n_requests 1 .. 4096.
+ * d_workspace: oxb_hip_paged_attention_workspace bytes (at the same counts, no GPU needed, pointers are not looked at), 256-byte
+ * aligned, contents of no meaning before and after; calls that overlap in time need one each. */
+typedef struct {
+    uint32_t n_tokens, n_requests, n_groups, nq, dtype, q_stride, out_stride, table_width;
+    const void* d_q;
+    void* d_out;
+    float* d_lse;
+    const int32_t *d_tables, *d_cu_tokens, *d_positions, *d_lens, *d_cu_groups, *d_prefix_lens;
+    float scale;
+    void* d_workspace;
+    size_t workspace_bytes;
+    oxb_page_pool pool;
+} oxb_paged_attention;
+int  oxb_hip_paged_attention_workspace(const oxb_paged_attention* a, size_t* n_bytes);
+int  oxb_hip_paged_attention_dev(const oxb_paged_attention* a);
+
 /* ---- the steps either side of the fused forward: checkpoint file -> device, token ids in, token ids out.
  * oxb_hip_gguf_info (no GPU needed) and oxb_hip_load_gguf read a GGUF file the way GgufFile::parse does
  * (crates/oxibonsai-core/src/gguf/reader.rs:11-80, header.rs, metadata.rs, tensor_info.rs) and assemble the model

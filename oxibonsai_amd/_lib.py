@@ -84,6 +84,10 @@ _SIGNATURES = {
     "oxb_hip_sum_in_order": ([f32p, C.c_uint32, f32p], C.c_int),
     "oxb_hip_set_gemv_packed_min_batch": ([C.c_uint32], C.c_int),
     "oxb_hip_prefill_tokens": ([C.c_uint64, C.c_uint64, C.c_uint32, u32p, C.c_uint32, C.c_uint32, f32p, u32p], C.c_int),
+    "oxb_hip_paged_assign_dev": ([C.c_void_p], C.c_int),
+    "oxb_hip_paged_rows_dev": ([C.c_void_p], C.c_int),
+    "oxb_hip_paged_attention_workspace": ([C.c_void_p, szp], C.c_int),
+    "oxb_hip_paged_attention_dev": ([C.c_void_p], C.c_int),
     "oxb_hip_host_alloc": ([C.POINTER(C.c_void_p), C.c_size_t], C.c_int),
     "oxb_hip_host_free": ([C.c_void_p], C.c_int),
     "oxb_hip_repack_sizes": ([C.c_int, C.c_uint32, C.c_uint32, szp, szp], C.c_int),

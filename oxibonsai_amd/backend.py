@@ -92,6 +92,10 @@ class NativeHipBackend:
     def synchronize(self, device_id: int = 0) -> None:
         _check(self._lib.oxb_hip_synchronize())
 
+    def set_stream(self, hip_stream: int = 0) -> None:
+        """Calls run on the caller's HIP stream from here on (``torch.cuda.Stream.cuda_stream``); 0 restores the library's own."""
+        _check(self._lib.oxb_hip_set_stream(hip_stream or None))
+
     def memory_info(self, device_id: int = 0) -> tuple[int, int]:
         """(free, total) bytes."""
         f, t = C.c_size_t(0), C.c_size_t(0)

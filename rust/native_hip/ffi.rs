@@ -107,6 +107,93 @@ pub struct OxbGgufInfo {
     pub lm_head_rows: u32,
 }
 
+/// One layer's rows of a paged cache on the device (`OXB_KV_DTYPE_*`).
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct OxbPagePool {
+    pub d_k: *mut c_void,
+    pub d_v: *mut c_void,
+    pub d_k_scale: *mut f32,
+    pub d_v_scale: *mut f32,
+    pub kv_dtype: u32,
+    pub nkv: u32,
+    pub hd: u32,
+    pub page_size: u32,
+    pub n_pages: u32,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct OxbPageAssign {
+    pub n_requests: u32,
+    pub page_size: u32,
+    pub n_pages: u32,
+    pub table_width: u32,
+    pub n_rows: u32,
+    pub d_past: *const i32,
+    pub d_keep: *const i32,
+    pub d_add: *const i32,
+    pub d_tables: *mut i32,
+    pub d_free_pages: *mut i32,
+    pub d_n_free: *const i32,
+    pub d_n_free_out: *mut i32,
+    pub d_lens: *mut i32,
+    pub d_cu_tokens: *mut i32,
+    pub d_cu_pages: *mut i32,
+    pub d_slots: *mut i32,
+    pub d_positions: *mut i32,
+    pub d_status: *mut i32,
+}
+
+/// Types of rows (`OXB_DTYPE_*`): 0 f32, 1 f16, 2 bf16.
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct OxbPagedRows {
+    pub n_rows: u32,
+    pub nq: u32,
+    pub d_qkv: *const c_void,
+    pub qkv_dtype: u32,
+    pub qkv_stride: u32,
+    pub d_positions: *const i32,
+    pub d_slots: *const i32,
+    pub d_q_norm: *const f32,
+    pub d_k_norm: *const f32,
+    pub d_cos: *const f32,
+    pub d_sin: *const f32,
+    pub n_angles: u32,
+    pub eps: f32,
+    pub d_q_out: *mut c_void,
+    pub q_dtype: u32,
+    pub q_stride: u32,
+    pub pool: OxbPagePool,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy)]
+pub struct OxbPagedAttention {
+    pub n_tokens: u32,
+    pub n_requests: u32,
+    pub n_groups: u32,
+    pub nq: u32,
+    pub dtype: u32,
+    pub q_stride: u32,
+    pub out_stride: u32,
+    pub table_width: u32,
+    pub d_q: *const c_void,
+    pub d_out: *mut c_void,
+    pub d_lse: *mut f32,
+    pub d_tables: *const i32,
+    pub d_cu_tokens: *const i32,
+    pub d_positions: *const i32,
+    pub d_lens: *const i32,
+    pub d_cu_groups: *const i32,
+    pub d_prefix_lens: *const i32,
+    pub scale: f32,
+    pub d_workspace: *mut c_void,
+    pub workspace_bytes: usize,
+    pub pool: OxbPagePool,
+}
+
 extern "C" {
     // lifecycle
     pub fn oxb_hip_init(device_ordinal: c_int) -> c_int;
@@ -182,6 +269,11 @@ extern "C" {
                                  tokens_out: *mut u32) -> c_int;
     pub fn oxb_hip_prefill_tokens(model: u64, embedding: u64, seq: u32, ids: *const u32, n_tokens: u32, pos_start: u32,
                                   logits_or_null: *mut f32, token_out_or_null: *mut u32) -> c_int;
+    // a serving step over a paged cache, on device buffers
+    pub fn oxb_hip_paged_assign_dev(a: *const OxbPageAssign) -> c_int;
+    pub fn oxb_hip_paged_rows_dev(a: *const OxbPagedRows) -> c_int;
+    pub fn oxb_hip_paged_attention_workspace(a: *const OxbPagedAttention, n_bytes: *mut usize) -> c_int;
+    pub fn oxb_hip_paged_attention_dev(a: *const OxbPagedAttention) -> c_int;
     // pinned host memory for results
     pub fn oxb_hip_host_alloc(p: *mut *mut c_void, n_bytes: usize) -> c_int;
     pub fn oxb_hip_host_free(p: *mut c_void) -> c_int;
