@@ -7,11 +7,15 @@
 // sum_parts exp(m_part - m) (l_part, o_part) is the whole.  So the prefix is read once for all queries of the group, the rows of
 // its products being all (query, q head) pairs of a kv head, and only the rests are read request by request.
 //
-// Work is cut on the device, because the lengths lie there: every workgroup sums up the work of all entries (an entry: a
-// group's prefix or a request's rest), which gives the number of keys that one item of work walks, then takes items
-// blockIdx.x, + gridDim.x, ...  An item is (entry, run of keys, tile of rows, kv head), kv head fastest: workgroups go to the
-// eight XCDs in turn, so the row tiles of one kv head and run meet in one L2.  Rows whose keys are all in one item are written
-// at once, the others' parts go to the workspace and a second launch adds them.
+// Work is cut on the device, because the lengths lie there.  An entry is a group's prefix or a request's rest, a unit one kv
+// head and tile of rows of an entry over all its keys, and the work of all units, laid end to end, is dealt out in equal shares, one
+// to a workgroup (512: two to a CU): every workgroup sums up the entries' work, finds where its share begins and walks from there,
+// the end of one unit, whole ones, the beginning of another.  A row whose unit lies in one share and has no other part is
+// written at once, other parts go to the workspace and a second launch adds them; there are at most 512 more parts than units.
+// Workgroups go to the eight XCDs in turn; shares go to them in runs, so that what is read more than once (the prefix, by
+// each tile of rows of a kv head) is read at about the same time through one L2.  The first workgroup of a CU takes from the
+// first half, where the prefixes are, which are bound by the matrix cores, the second one from the second half, where the rests
+// are, which are bound by memory.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -24,21 +28,33 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 
-#define PA_BLOCK 32u       // keys of a block: what one wave scores at a time
-#define PA_TILE 16u        // rows of an item
-#define PA_GRID 512u       // workgroups: two to a CU
-#define PA_TARGET 1024u    // items that the work of a call is cut into, about
-#define PA_MIN_BLOCKS 4u   // blocks of an item, at least: one for each wave
+#define PA_SHARES 512u     // workgroups: two to a CU
+#define PA_FEW 32u         // rows up to which an entry's tiles have 16 rows and its waves take the keys in turn
+#define PA_TILE_FEW 16u
+#define PA_KEYS_FEW 128u   // keys that a workgroup takes at a time: 32 by each wave
 #define PA_LOG2E 1.44269504088896340736f
+
+// Tiles of many rows and the keys of a block of theirs: what the registers and two workgroups' LDS hold.
+constexpr uint32_t pa_tile_many(uint32_t hd) { return hd == 256 ? 64u : 128u; }
+constexpr uint32_t pa_keys_many(uint32_t hd) { return hd == 256 ? 32u : 64u; }
+
+// Work, in units that mean nothing but relative to each other: a block of keys for few rows (a wait for memory), for many rows
+// (products), and what a unit costs whatever its keys are.
+struct PaCosts {
+    uint32_t few, many, unit;
+};
 
 struct PaParams {
     oxb_paged_attention a;
-    float scale_log2;  // scale * log2 e
+    float scale_log2;  // |scale| * log2 e
+    uint32_t negative; // the scale's sign bit, for q
     uint32_t G;        // q heads to a kv head
     uint32_t page_shift;
-    uint4* entries;    // workspace: what the merge needs of every entry: first part, chunks (0: no parts), rows of a kv head, first token
-    float2* ml;        // maximum (log2 units) and sum of every part
-    float* o;          // [parts][hd]
+    uint32_t tile_many, keys_many;
+    PaCosts cost;
+    struct PaLeft* entries;  // workspace: what the merge needs of every entry; [n_groups + n_requests] is the share
+    float2* ml;        // maximum (log2 units) and sum of every part's rows
+    float* o;          // [rows of parts][hd]
 };
 
 struct PaEntry {
@@ -47,6 +63,20 @@ struct PaEntry {
     uint32_t table;     // row of the page tables
     bool parts;         // the rows have another part elsewhere
     bool bad;           // sums that do not ascend
+};
+
+// How an entry is cut.
+struct PaCut {
+    uint32_t rows, tile, tiles;     // rows of a kv head, of a tile; tiles
+    uint32_t keys, b0, blocks;      // keys of a block; the first block; how many
+    uint32_t block, unit;           // work of a block, of a unit
+};
+
+// What the attention leaves for the merge.
+struct PaLeft {
+    unsigned long long w0;          // where the entry's work begins
+    uint32_t row0;                  // ... and its rows of parts
+    uint32_t rows, tile, tiles, blocks, block, unit, t0, parts, pad;
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
@@ -95,151 +125,137 @@ __device__ __forceinline__ PaEntry pa_entry(const oxb_paged_attention& a, uint32
     x.tn = t1 > x.t0 ? t1 - x.t0 : 0u;
     return x;
 }
-__device__ __forceinline__ uint32_t pa_tiles(const PaEntry& x, uint32_t G) { return (x.tn * G + PA_TILE - 1) / PA_TILE; }
-__device__ __forceinline__ uint32_t pa_blocks(const PaEntry& x) {  // (a rest without keys is one block, in which nothing is seen)
-    const uint32_t b = x.k1 > x.k0 ? (x.k1 + PA_BLOCK - 1) / PA_BLOCK - x.k0 / PA_BLOCK : 0u;
-    return b ? b : 1u;
+__device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x) {
+    PaCut c;
+    c.rows = x.tn * p.G;
+    const bool few = c.rows <= PA_FEW;
+    c.tile = few ? PA_TILE_FEW : p.tile_many;
+    c.keys = few ? PA_KEYS_FEW : p.keys_many;
+    c.block = few ? p.cost.few : p.cost.many;
+    c.tiles = (c.rows + c.tile - 1) / c.tile;
+    c.b0 = x.k0 / c.keys;
+    c.blocks = x.k1 > x.k0 ? (x.k1 + c.keys - 1) / c.keys - c.b0 : 1u;  // (a rest without keys is one block, in which nothing is seen)
+    c.unit = p.cost.unit + c.blocks * c.block;
+    return c;
 }
-// Blocks of an item of this entry, about `each` of them: equal shares.
-__device__ __forceinline__ uint32_t pa_chunks(uint32_t blocks, uint32_t each, uint32_t& per) {
-    const uint32_t n = (blocks + each - 1) / each;
-    per = (blocks + n - 1) / n;
-    return (blocks + per - 1) / per;
+// a / b; the numbers of nearly all calls have 32 bits
+__device__ __forceinline__ uint32_t pa_div(unsigned long long a, unsigned long long b) {
+    return (uint32_t)(((a | b) >> 32) == 0 ? (uint32_t)a / (uint32_t)b : a / b);
 }
-
-struct PaItem {
-    PaEntry x;
-    uint32_t rows, chunk, tile, kvh;
-    uint32_t b0, b1;     // blocks of keys, counted from position 0
-    uint32_t part0;      // first part of the entry
-    bool parts;
-};
 
 // What a workgroup knows about the whole call: its threads hold a run of entries each.
 struct PaPlan {
-    uint32_t each;              // blocks of an item, about
-    uint32_t items;
+    unsigned long long work, share;
     uint32_t e0, e1;            // this thread's entries
-    uint32_t item0, part0;      // ... and the first item and part of them
+    unsigned long long w0;      // ... and where their work
+    uint32_t row0;              // ... and rows of parts begin
+};
+struct PaAt {                   // an entry in which a share has work
+    PaEntry x;
+    PaCut c;
+    unsigned long long w0;
+    uint32_t row0, unit;        // the unit in which the work begins
 };
 struct PaPlanLds {
     unsigned long long work[4];
-    uint32_t bad[4];
-    uint32_t items[4], parts[4];
-    PaItem item;
+    uint32_t rows[4], bad[4], most[4];
+    PaAt at;
 };
 
-// One item's cost in blocks is the same for all, so equal runs of keys are equal work.
 __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, bool leave_entries) {
     const oxb_paged_attention& a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_groups + a.n_requests, per = (E + 255u) / 256u;
     PaPlan pl;
     pl.e0 = min(tid * per, E);
     pl.e1 = min(pl.e0 + per, E);
-    PaEntry first = {0, 0, 0, 0, 0, false, false};
     unsigned long long work = 0;
+    uint32_t rows = 0;
     bool bad = false;
     for (uint32_t e = pl.e0; e < pl.e1; e++) {
         const PaEntry x = pa_entry(a, e);
-        if (e == pl.e0) first = x;
+        const PaCut c = pa_cut(p, x);
         bad |= x.bad;
-        work += (unsigned long long)pa_tiles(x, p.G) * a.pool.nkv * pa_blocks(x);
+        work += (unsigned long long)c.unit * c.tiles * a.pool.nkv;
+        rows += c.rows * a.pool.nkv;
     }
-#pragma unroll
-    for (int d = 32; d; d /= 2) work += __shfl_xor(work, d, 64);
-    // (with sums that do not ascend the parts could pass the workspace: nothing is done at all)
-    bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-    if (lane == 0) lds.work[wave] = work, lds.bad[wave] = bad;
-    __syncthreads();
-    bad = lds.bad[0] | lds.bad[1] | lds.bad[2] | lds.bad[3];
-    if (bad) pl.e1 = pl.e0;
-    work = lds.work[0] + lds.work[1] + lds.work[2] + lds.work[3];
-    const unsigned long long each = (work + PA_TARGET - 1) / PA_TARGET;
-    pl.each = (uint32_t)min(max(each, (unsigned long long)PA_MIN_BLOCKS), 0x7FFFFFFFull);
-    uint32_t items = 0, parts = 0;
-    auto count = [&](uint32_t e, uint32_t& n_parts, uint32_t& n_chunks, PaEntry& x) -> uint32_t {
-        x = e == pl.e0 ? first : pa_entry(a, e);
-        uint32_t run;
-        n_chunks = pa_chunks(pa_blocks(x), pl.each, run);
-        n_parts = x.parts || n_chunks > 1 ? x.tn * p.G * a.pool.nkv * n_chunks : 0u;
-        return pa_tiles(x, p.G) * a.pool.nkv * n_chunks;
-    };
-    for (uint32_t e = pl.e0; e < pl.e1; e++) {
-        uint32_t np, nc;
-        PaEntry x;
-        items += count(e, np, nc, x);
-        parts += np;
-    }
-    uint32_t ii = items, ip = parts;
+    unsigned long long iw = work;
+    uint32_t ir = rows;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-        const uint32_t oi = __shfl_up(ii, d, 64), op = __shfl_up(ip, d, 64);
-        if (lane >= (uint32_t)d) ii += oi, ip += op;
+        const unsigned long long ow = __shfl_up(iw, d, 64);
+        const uint32_t orr = __shfl_up(ir, d, 64);
+        if (lane >= (uint32_t)d) iw += ow, ir += orr;
     }
-    if (lane == 63) lds.items[wave] = ii, lds.parts[wave] = ip;
+    bad = __builtin_amdgcn_ballot_w64(bad) != 0;
+    if (lane == 63) lds.work[wave] = iw, lds.rows[wave] = ir, lds.bad[wave] = bad;
     __syncthreads();
-    pl.item0 = ii - items;
-    pl.part0 = ip - parts;
-    pl.items = 0;
+    pl.w0 = iw - work;
+    pl.row0 = ir - rows;
+    pl.work = 0;
+    bad = false;
     for (uint32_t w = 0; w < 4; w++) {
-        if (w < wave) pl.item0 += lds.items[w], pl.part0 += lds.parts[w];
-        pl.items += lds.items[w];
+        if (w < wave) pl.w0 += lds.work[w], pl.row0 += lds.rows[w];
+        pl.work += lds.work[w];
+        bad |= lds.bad[w] != 0;
     }
+    // (no share without a block: parts are counted by the blocks that begin in a share)
+    pl.share = max((pl.work + PA_SHARES - 1) / PA_SHARES, (unsigned long long)max(p.cost.few, p.cost.many));
+    // (with sums that do not ascend the parts could pass the workspace: nothing is done at all)
+    if (bad) pl.work = 0;
     if (leave_entries) {
-        if (bad)
-            for (uint32_t e = tid; e < E; e += 256) p.entries[e] = make_uint4(0, 0, 0, 0);
-        uint32_t at = pl.part0;
+        unsigned long long w = pl.w0;
+        uint32_t row = pl.row0;
         for (uint32_t e = pl.e0; e < pl.e1; e++) {
-            uint32_t np, nc;
-            PaEntry x;
-            count(e, np, nc, x);
-            p.entries[e] = make_uint4(at, np ? nc : 0u, x.tn * p.G, x.t0);
-            at += np;
+            const PaEntry x = pa_entry(a, e);
+            const PaCut c = pa_cut(p, x);
+            p.entries[e] = {w, row, bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.block, c.unit, x.t0, x.parts, 0};
+            w += (unsigned long long)c.unit * c.tiles * a.pool.nkv;
+            row += c.rows * a.pool.nkv;
         }
+        if (tid == 0) p.entries[E].w0 = pl.share;
     }
     return pl;
 }
 
-// Item i, worked out by the thread that holds its entry and left in LDS for all (two barriers).
-__device__ __forceinline__ PaItem pa_item(const PaParams& p, const PaPlan& pl, PaPlanLds& lds, uint32_t i) {
+// The entry in which the work at w lies, found by the thread that holds it and left in LDS for all (two barriers).
+__device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, PaPlanLds& lds, unsigned long long w) {
     const oxb_paged_attention& a = p.a;
-    uint32_t at = pl.item0, part = pl.part0;
+    unsigned long long at = pl.w0;
+    uint32_t row = pl.row0;
     __syncthreads();
-    if (i >= at)
+    if (w >= at)
         for (uint32_t e = pl.e0; e < pl.e1; e++) {
             const PaEntry x = pa_entry(a, e);
-            const uint32_t blocks = pa_blocks(x), tiles = pa_tiles(x, p.G);
-            uint32_t run;
-            const uint32_t chunks = pa_chunks(blocks, pl.each, run), n = tiles * a.pool.nkv * chunks;
-            const bool parts = x.parts || chunks > 1;
-            if (i - at < n) {
-                PaItem it;
-                const uint32_t j = i - at;
-                it.x = x;
-                it.kvh = j % a.pool.nkv;
-                it.tile = j / a.pool.nkv % tiles;
-                it.chunk = j / a.pool.nkv / tiles;
-                it.rows = x.tn * p.G;
-                it.b0 = x.k0 / PA_BLOCK + it.chunk * run;
-                it.b1 = min(it.b0 + run, x.k0 / PA_BLOCK + blocks);
-                it.part0 = part;
-                it.parts = parts;
-                lds.item = it;
+            const PaCut c = pa_cut(p, x);
+            const unsigned long long n = (unsigned long long)c.unit * c.tiles * a.pool.nkv;
+            if (w - at < n) {
+                lds.at = {x, c, at, row, pa_div(w - at, c.unit)};
                 break;
             }
             at += n;
-            part += parts ? x.tn * p.G * a.pool.nkv * chunks : 0u;
+            row += c.rows * a.pool.nkv;
         }
     __syncthreads();
-    PaItem it = lds.item;  // the same for all: into scalar registers
-    it.x.t0 = uniform(it.x.t0), it.x.k0 = uniform(it.x.k0), it.x.k1 = uniform(it.x.k1), it.x.table = uniform(it.x.table);
-    it.rows = uniform(it.rows), it.chunk = uniform(it.chunk), it.tile = uniform(it.tile), it.kvh = uniform(it.kvh);
-    it.b0 = uniform(it.b0), it.b1 = uniform(it.b1), it.part0 = uniform(it.part0), it.parts = uniform(it.parts) != 0;
-    return it;
+    PaAt r = lds.at;  // the same for all: into scalar registers
+    r.x.t0 = uniform(r.x.t0), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1), r.x.table = uniform(r.x.table), r.x.parts = uniform(r.x.parts) != 0;
+    r.c.rows = uniform(r.c.rows), r.c.tile = uniform(r.c.tile), r.c.tiles = uniform(r.c.tiles), r.c.b0 = uniform(r.c.b0);
+    r.c.blocks = uniform(r.c.blocks), r.c.block = uniform(r.c.block), r.c.unit = uniform(r.c.unit), r.c.keys = uniform(r.c.keys);
+    r.row0 = uniform(r.row0), r.unit = uniform(r.unit);
+    r.w0 = (unsigned long long)uniform((uint32_t)(r.w0 >> 32)) << 32 | uniform((uint32_t)r.w0);
+    return r;
 }
 
-// Eight values of q from memory, as fp32.
-__device__ __forceinline__ void pa_load_q8(const void* q, uint32_t dtype, size_t at, float v[8]) {
+// What a workgroup does at a time: blocks b0 .. b1 of a tile of an entry's rows.
+struct PaItem {
+    PaEntry x;
+    uint32_t rows, row0, kvh;  // rows of a kv head; the tile's first
+    uint32_t b0, b1;
+    size_t part;               // where the tile's rows of parts begin
+    bool parts;
+};
+
+// Eight values of q from memory, as fp32, times the scale's sign.
+__device__ __forceinline__ void pa_load_q8(const void* q, uint32_t dtype, uint32_t sign, size_t at, float v[8]) {
     if (dtype == OXB_DTYPE_F32) {
         const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q) + at);
         const float4 x = s[0], y = s[1];
@@ -252,6 +268,8 @@ __device__ __forceinline__ void pa_load_q8(const void* q, uint32_t dtype, size_t
             v[i] = dtype == OXB_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : __uint_as_float(b << 16);
         }
     }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = __uint_as_float(__float_as_uint(v[i]) ^ sign);
 }
 __device__ __forceinline__ uint32_t pa_bits16(float v, uint32_t dtype) {
     if (dtype == OXB_DTYPE_F16) return __builtin_bit_cast(uint16_t, (_Float16)v);
@@ -270,7 +288,7 @@ __device__ __forceinline__ void pa_store4(void* out, uint32_t dtype, size_t at, 
 __device__ __forceinline__ float pa_lse(float m, float l) { return l > 0.f ? (m + log2f(l)) * 0.693147180559945309417f : l == 0.f ? -INFINITY : NAN; }
 
 // ---------------------------------------------------------------------------
-// Few rows: a request's rest, a small group's prefix.  16 rows, the four waves take the item's blocks of 32 keys in turn and add their
+// Few rows: a request's rest, a small group's prefix.  16 rows, the four waves take 32 keys each of a block of 128 and add their
 // sums in LDS at the end; operands come from memory straight into registers, the next block's while this one is worked on.
 //
 // Products as in the prefill attention, transposed, on v_mfma_f32_16x16x32_f16: S^T = K Q^T leaves a lane (row c = lane % 16,
@@ -321,7 +339,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
     const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
     const uint32_t wave = uniform(tid >> 6);
     // this lane's row
-    const uint32_t row = it.tile * PA_TILE + c;
+    const uint32_t row = it.row0 + c;
     const bool there = row < it.rows;
     const uint32_t tok = it.x.t0 + (there ? row : it.rows - 1) / p.G, head = it.kvh * p.G + (there ? row : it.rows - 1) % p.G;
     const int pos = a.d_positions[tok];
@@ -335,7 +353,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
     most = uniform(most);
     least = uniform(least);
     const uint32_t lo = it.x.k0, kvh = it.kvh;
-    const uint32_t b1 = most > lo ? min(it.b1, (most + PA_BLOCK - 1) / PA_BLOCK) : 0u;  // (nothing is seen behind)
+    const uint32_t b1 = most > lo ? min(4 * it.b1, (most + 31u) / 32u) : 0u;  // (nothing is seen behind)
 
     // q: element e of step s is dimension dim(s) + e
     auto dim = [&](int s) -> uint32_t { return QC && KS > 1 ? 64u * (s / 2) + 16u * g + 8u * (s % 2) : 32u * s + 8u * g; };
@@ -345,13 +363,13 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
         float f[KS][8], top = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            pa_load_q8(a.d_q, a.dtype, (size_t)tok * a.q_stride + (size_t)head * HD + dim(s), f[s]);
+            pa_load_q8(a.d_q, a.dtype, p.negative, (size_t)tok * a.q_stride + (size_t)head * HD + dim(s), f[s]);
 #pragma unroll
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[s][e]));
         }
         top = max_rows4(top);
         const int ex = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-        mul = __builtin_amdgcn_ldexpf(p.scale_log2, ex);
+        mul = __builtin_amdgcn_ldexpf(p.scale_log2, ex);  // (the sign is q's)
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll
@@ -377,7 +395,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
             // rows in front of the first key or behind the last one that is seen are not read: they need hold no numbers
-            const uint32_t at = max(min(b * PA_BLOCK + 16 * kt, last & ~15u), lo & ~15u), from = lo > at ? min(lo - at, 15u) : 0u, to = min(last - at, 15u);
+            const uint32_t at = max(min(b * 32u + 16 * kt, last & ~15u), lo & ~15u), from = lo > at ? min(lo - at, 15u) : 0u, to = min(last - at, 15u);
             const size_t r = row_of(at);
             const uint8_t *kr = Kc + r * ROWB, *vr = Vc + r * ROWB;
             const uint32_t kc = max(min(c, to), min(from, to)) * ROWB;
@@ -417,8 +435,8 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
                 for (int t = 0; t < TERMS; t++) S[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K, q[t][s], S[kt], 0, 0, 0);
             }
         float vs[2][4], top = -INFINITY;
-        const uint32_t key0 = b * PA_BLOCK;
-        const bool all = key0 >= lo && key0 + PA_BLOCK <= least;  // (wave-uniform) every row sees all of these keys
+        const uint32_t key0 = b * 32u;
+        const bool all = key0 >= lo && key0 + 32u <= least;  // (wave-uniform) every row sees all of these keys
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
@@ -491,7 +509,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
     };
     // (two blocks of wide rows do not fit the registers)
     constexpr bool AHEAD = HD < 256;
-    const uint32_t b0 = it.b0 + wave;
+    const uint32_t b0 = 4 * it.b0 + wave;
     if constexpr (AHEAD) {
         Block A, B;
         if (b0 < b1) request(A, b0);
@@ -523,7 +541,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
         for (int j = 0; j < DPL; j++) lo_o[(wave * 16 + c) * LD + (4 * g + v) * DPL + j] = O[j][v];
     __syncthreads();
     // row r of the tile by 16 threads, HD / 16 dimensions each: four at a time, 64 apart
-    const uint32_t r = tid >> 4, u = tid & 15u, out_row = it.tile * PA_TILE + r;
+    const uint32_t r = tid >> 4, u = tid & 15u, out_row = it.row0 + r;
     if (out_row >= it.rows) return;
     float2 w[4];
     float top = -INFINITY, sum = 0.f, f[4];
@@ -533,7 +551,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
 #pragma unroll
     for (int i = 0; i < 4; i++) f[i] = __builtin_amdgcn_exp2f(w[i].x - ref), sum = fmaf(w[i].y, f[i], sum);
     const uint32_t t = it.x.t0 + out_row / p.G, h = it.kvh * p.G + out_row % p.G;
-    const size_t part = (size_t)it.part0 + ((size_t)it.chunk * a.pool.nkv + it.kvh) * it.rows + out_row;
+    const size_t part = it.part + r;
     const float inv = it.parts ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
     constexpr uint32_t STEP = HD < 64 ? HD : 64;
     if (4 * u < STEP)
@@ -556,20 +574,348 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
     }
 }
 
+// ---------------------------------------------------------------------------
+// Many rows: a large group's prefix, a prompt's chunk.  A wave has QT tiles of 16 rows, the four walk the same blocks of keys, K and
+// V, which lie in LDS as fp16 rows, twice: the next block is on its way while one is worked on.  fp16 rows go there directly,
+// one-byte rows wait in registers and are widened on their way.  The rows' 16-byte pieces are permuted by an XOR with the
+// row number, so that neither the reads of K (16 rows, one piece) nor the transposing reads of V meet in a bank.
+//
+// The same products and softmax as above; V's operand comes from the transposing reads.  Bound by the matrix cores, the LDS
+// reads (two tiles share an operand) and the VALU's softmax about equally: 512 cycles each per 32 keys of head_dim 128 and
+// wave.
+// ---------------------------------------------------------------------------
+template <int HD>
+constexpr int pa_many_lds_halves() {
+    return 4 * (int)pa_keys_many(HD) * HD;
+}
+
+template <int HD, int KVM, int TERMS, int QT>
+__device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it, PaPlanLds& plan_lds, _Float16* lds, float* scales) {
+    constexpr bool QC = KVM != OXB_KV_F16;
+    constexpr int KB = (int)pa_keys_many(HD), KS = HD / 32, NS = HD / 16, NT = KB / 16, NH = KB / 32;
+    constexpr uint32_t ROWB = HD * (QC ? 1 : 2);
+    constexpr int PPR = HD / 8, RPW = KB / 4;                       // pieces of an LDS row; rows that a wave fetches
+    constexpr int RB = PPR >= 16 ? 1 : 16 / PPR, PM = (PPR < 16 ? PPR : 16) - 1;  // rows of 256 bytes; the permutation's mask
+    constexpr int NI = (RPW * (int)ROWB / 16 + 63) / 64;            // 16-byte pieces per lane and block, of K and of V
+    constexpr bool HALF = RPW * ROWB / 16 < 64;                     // half a wave holds them all
+    const oxb_paged_attention& a = p.a;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
+    const uint32_t wave = uniform(tid >> 6);
+    const uint32_t lo = it.x.k0, kvh = it.kvh;
+
+    uint32_t tok[QT], head[QT], sees[QT], most = 0, least = 0xFFFFFFFFu;
+    bool there[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const uint32_t row = it.row0 + (t * 4 + wave) * 16 + c, r = min(row, it.rows - 1);
+        there[t] = row < it.rows;
+        tok[t] = it.x.t0 + r / p.G;
+        head[t] = kvh * p.G + r % p.G;
+        const int pos = a.d_positions[tok[t]];
+        sees[t] = min(pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), it.x.k1);
+        most = max(most, there[t] ? sees[t] : 0u);
+        least = min(least, there[t] ? sees[t] : 0xFFFFFFFFu);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+        most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+        least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
+    }
+    most = uniform(most);
+    least = uniform(least);
+    __syncthreads();
+    if (lane == 0) plan_lds.most[wave] = most;
+    __syncthreads();
+    const uint32_t wg_most = uniform(max(max(plan_lds.most[0], plan_lds.most[1]), max(plan_lds.most[2], plan_lds.most[3])));
+    const uint32_t last = wg_most - 1;
+    const uint32_t b1 = wg_most > lo ? min(it.b1, last / KB + 1) : 0u;
+
+    // q as in the other form; element e of step s is dimension 32 s + 8 g + e
+    v8h q[TERMS][QT][KS];
+    float mul[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        float f[KS][8], top = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            pa_load_q8(a.d_q, a.dtype, p.negative, (size_t)tok[t] * a.q_stride + (size_t)head[t] * HD + 32 * s + 8 * g, f[s]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[s][e]));
+        }
+        top = max_rows4(top);
+        const int ex = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+        mul[t] = __builtin_amdgcn_ldexpf(p.scale_log2, ex);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = __builtin_amdgcn_ldexpf(f[s][e], -ex);
+                const _Float16 hi = (_Float16)x;
+                q[0][t][s][e] = hi;
+                if constexpr (TERMS == 2) q[1][t][s][e] = (_Float16)(x - (float)hi);
+            }
+    }
+
+    typedef const __attribute__((address_space(4))) int32_t* ConstInts;
+    const ConstInts table = (ConstInts)(uintptr_t)(a.d_tables + (size_t)it.x.table * a.table_width);
+    const uint8_t* const Kc = reinterpret_cast<const uint8_t*>(a.pool.d_k);
+    const uint8_t* const Vc = reinterpret_cast<const uint8_t*>(a.pool.d_v);
+    _Float16 *const ks0 = lds, *const vs0 = lds + KB * HD, *const ks1 = lds + 2 * KB * HD, *const vs1 = lds + 3 * KB * HD;
+    // this wave's rows of block b: positions `at` .. in one page; those in front of the first key or behind the last one are not read
+    auto rows_of = [&](uint32_t b, uint32_t& from, uint32_t& to) -> size_t {
+        const uint32_t at = max(min(b * KB + wave * RPW, last & ~(uint32_t)(RPW - 1)), lo & ~(uint32_t)(RPW - 1));
+        to = min(last - at, (uint32_t)RPW - 1);
+        from = min(lo > at ? lo - at : 0u, to);
+        const uint32_t page = (uint32_t)table[at >> p.page_shift], safe = min(page, a.pool.n_pages - 1);
+        return (((size_t)kvh * a.pool.n_pages + safe) << p.page_shift) + (at & (a.pool.page_size - 1u));
+    };
+    v4w kreg[QC ? NI : 1], vreg[QC ? NI : 1];
+    float kscale = 0.f, vscale = 0.f;
+    auto request = [&](uint32_t b, _Float16* kd, _Float16* vd) {
+        uint32_t from, to;
+        const size_t row = rows_of(b, from, to);
+        const uint8_t *kb = Kc + row * ROWB, *vb = Vc + row * ROWB;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            constexpr uint32_t SPR = ROWB / 16;  // pieces of a cache row
+            const uint32_t id = i * 64 + lane, r = id / SPR, piece = QC ? id % SPR : (id % SPR) ^ (((wave * RPW + r) / RB) & PM);
+            const uint32_t off = max(min(r, to), from) * ROWB + piece * 16;
+            if constexpr (QC) {
+                if (!HALF || lane < RPW * ROWB / 16) {
+                    kreg[i] = *reinterpret_cast<const v4w*>(kb + off);
+                    vreg[i] = *reinterpret_cast<const v4w*>(vb + off);
+                }
+            } else {
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + off),
+                                                 (__attribute__((address_space(3))) void*)(kd + (wave * RPW * PPR + i * 64) * 8), 16, 0, 0);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + off),
+                                                 (__attribute__((address_space(3))) void*)(vd + (wave * RPW * PPR + i * 64) * 8), 16, 0, 0);
+            }
+        }
+        if constexpr (QC) {
+            const uint32_t r = max(min(lane & (RPW - 1), to), from);
+            kscale = a.pool.d_k_scale[row + r];
+            vscale = a.pool.d_v_scale[row + r];
+        }
+    };
+    // The barrier that ends a block: every wave has read it, and the next one is complete in LDS.
+    auto deliver = [&](_Float16* kd, _Float16* vd, float* sc, bool there_is) {
+        if (QC && there_is) {
+#pragma unroll
+            for (int i = 0; i < NI; i++) {
+                if (HALF && lane >= RPW * ROWB / 16) continue;
+                constexpr uint32_t SPR = ROWB / 16;
+                const uint32_t id = i * 64 + lane, r = wave * RPW + id / SPR, x = (r / RB) & PM, piece = 2 * (id % SPR);
+                uint32_t kw[8], vw[8];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    kv_dec4<KVM>(kreg[i][e], kw[2 * e], kw[2 * e + 1]);
+                    kv_dec4<KVM>(vreg[i][e], vw[2 * e], vw[2 * e + 1]);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const uint32_t at = (r * PPR + ((piece + e) ^ x)) * 8;
+                    *reinterpret_cast<v4w*>(kd + at) = (v4w){kw[4 * e], kw[4 * e + 1], kw[4 * e + 2], kw[4 * e + 3]};
+                    *reinterpret_cast<v4w*>(vd + at) = (v4w){vw[4 * e], vw[4 * e + 1], vw[4 * e + 2], vw[4 * e + 3]};
+                }
+            }
+            if (lane < RPW) sc[wave * RPW + lane] = kscale, sc[KB + wave * RPW + lane] = vscale;
+        }
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+
+    // K operand of step 0 in the first 16 keys, V operand of the first 16 dimensions in the first 16 keys (halves); step s and
+    // dimension tile sl are an XOR away
+    const uint32_t k_at = (c * PPR + (g ^ ((c / RB) & PM))) * 8;
+    const uint32_t v_row = 4 * g + (c >> 2), v_at = (v_row * PPR + (((c >> 1) & 1u) ^ ((v_row / RB) & PM))) * 8 + (c & 1u) * 4;
+    v4f O[QT][NS];
+    float m[QT], l[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+#pragma unroll
+        for (int i = 0; i < NS; i++) O[t][i] = (v4f){0.f, 0.f, 0.f, 0.f};
+        m[t] = -INFINITY;
+        l[t] = 0.f;
+    }
+    auto block = [&](const _Float16* kb, const _Float16* vb, const float* sc, uint32_t b) {
+        const uint32_t key0 = b * KB;
+        if (key0 >= most) return;  // (wave-uniform) nothing for this wave's rows
+        v4f S[QT][NT];
+#pragma unroll
+        for (int hb = 0; hb < NH; hb++) {
+            v8h K[2][KS];
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int kt = 0; kt < 2; kt++) K[kt][s] = *reinterpret_cast<const v8h*>(kb + (k_at ^ (32u * s)) + (2 * hb + kt) * 16 * HD);
+#pragma unroll
+            for (int t = 0; t < QT; t++) S[t][2 * hb] = S[t][2 * hb + 1] = (v4f){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int n = 0; n < TERMS; n++)
+#pragma unroll
+                    for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                        for (int t = 0; t < QT; t++) S[t][2 * hb + kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K[kt][s], q[n][t][s], S[t][2 * hb + kt], 0, 0, 0);
+        }
+        const bool all = key0 >= lo && key0 + KB <= least;  // (wave-uniform) every row sees all of these keys
+        v8h P[TERMS][QT][NH];
+        float vs[NT][4];
+#pragma unroll
+        for (int kt = 0; kt < NT; kt++) {
+            if constexpr (QC) {
+                const float4 x = *reinterpret_cast<const float4*>(sc + 16 * kt + 4 * g), y = *reinterpret_cast<const float4*>(sc + KB + 16 * kt + 4 * g);
+                const float k4[4] = {x.x, x.y, x.z, x.w}, v4[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    vs[kt][v] = v4[v];
+#pragma unroll
+                    for (int t = 0; t < QT; t++) S[t][kt][v] *= k4[v];
+                }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            if (!all) {
+#pragma unroll
+                for (int kt = 0; kt < NT; kt++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) {
+                        const uint32_t key = key0 + 16 * kt + 4 * g + v;
+                        S[t][kt][v] = key >= lo && key < sees[t] ? S[t][kt][v] : -INFINITY;
+                    }
+            }
+            float top = -INFINITY;
+#pragma unroll
+            for (int kt = 0; kt < NT; kt++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    if constexpr (QC) top = fmaxf(top, fmaf(S[t][kt][v], mul[t], (float)((int)(max(__float_as_uint(vs[kt][v]) & 0x7FFFFFFFu, 27u << 23) >> 23) - 127)));
+                    else top = fmaxf(top, S[t][kt][v]);
+                }
+            top = max_rows4(top);
+            if constexpr (!QC) top *= mul[t];
+            if (__builtin_amdgcn_ballot_w64(top > m[t])) {
+                const float now = fmaxf(top, m[t]), by = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
+                m[t] = now;
+                l[t] *= by;
+#pragma unroll
+                for (int i = 0; i < NS; i++)
+#pragma unroll
+                    for (int v = 0; v < 4; v++) O[t][i][v] *= by;
+            }
+            const float ref = m[t] == -INFINITY ? 0.f : m[t];
+            float sum = 0.f;
+#pragma unroll
+            for (int kt = 0; kt < NT; kt++)
+#pragma unroll
+                for (int v = 0; v < 4; v++) {
+                    float x = __builtin_amdgcn_exp2f(fmaf(S[t][kt][v], mul[t], -ref));
+                    sum += x;
+                    if constexpr (QC) {
+                        x *= vs[kt][v];
+                        if constexpr (TERMS == 2) asm("" : "+v"(x));  // (see above)
+                    }
+                    const _Float16 hi = (_Float16)x;
+                    P[0][t][kt / 2][4 * (kt % 2) + v] = hi;
+                    if constexpr (TERMS == 2) P[1][t][kt / 2][4 * (kt % 2) + v] = (_Float16)(x - (float)hi);
+                }
+            l[t] += sum;
+        }
+#pragma unroll
+        for (int hb = 0; hb < NH; hb++)
+#pragma unroll
+            for (int i = 0; i < NS; i++) {
+                const _Float16* tile = vb + (v_at ^ (16u * i)) + hb * 32 * HD;
+                const v4h_t t0 = lds_read_tr16(tile), t1 = lds_read_tr16(tile + 16 * HD);
+                const v8h V = {t0[0], t0[1], t0[2], t0[3], t1[0], t1[1], t1[2], t1[3]};
+#pragma unroll
+                for (int n = 0; n < TERMS; n++)
+#pragma unroll
+                    for (int t = 0; t < QT; t++) O[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V, P[n][t][hb], O[t][i], 0, 0, 0);
+            }
+    };
+    float *const sc0 = scales, *const sc1 = scales + 2 * KB;
+    if (it.b0 < b1) {
+        request(it.b0, ks0, vs0);
+        deliver(ks0, vs0, sc0, true);
+        for (uint32_t b = it.b0;;) {
+            if (b + 1 < b1) request(b + 1, ks1, vs1);
+            block(ks0, vs0, sc0, b);
+            if (++b >= b1) break;
+            deliver(ks1, vs1, sc1, true);
+            if (b + 1 < b1) request(b + 1, ks0, vs0);
+            block(ks1, vs1, sc1, b);
+            if (++b >= b1) break;
+            deliver(ks0, vs0, sc0, true);
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const float sum = sum_rows4(l[t]);
+        if (!there[t]) continue;
+        const size_t part = it.part + (t * 4 + wave) * 16 + c;
+        const float inv = it.parts ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < NS; i++) {
+            const float o[4] = {O[t][i][0] * inv, O[t][i][1] * inv, O[t][i][2] * inv, O[t][i][3] * inv};
+            if (it.parts) *reinterpret_cast<float4*>(p.o + part * HD + 16 * i + 4 * g) = make_float4(o[0], o[1], o[2], o[3]);
+            else pa_store4(a.d_out, a.dtype, (size_t)tok[t] * a.out_stride + (size_t)head[t] * HD + 16 * i + 4 * g, o);
+        }
+        if (g == 0) {
+            if (it.parts) p.ml[part] = make_float2(m[t], sum);
+            else if (a.d_lse) a.d_lse[(size_t)tok[t] * a.nq + head[t]] = pa_lse(m[t], sum);
+        }
+    }
+}
+
 template <int HD, int KVM, int TERMS>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PaParams p) {
+    constexpr int FEW = (4 * 16 * (HD + 4) + 4 * 16 * 2) * 4, MANY = pa_many_lds_halves<HD>() * 2 + 4 * (int)pa_keys_many(HD) * 4;
     __shared__ PaPlanLds plan_lds;
-    __shared__ __attribute__((aligned(16))) float lds[4 * 16 * (HD + 4) + 4 * 16 * 2];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[FEW > MANY ? FEW : MANY];
+    const oxb_paged_attention& a = p.a;
     const PaPlan pl = pa_plan(p, plan_lds, blockIdx.x == 0);
-    for (uint32_t i = blockIdx.x; i < pl.items; i += gridDim.x) {
-        const PaItem it = pa_item(p, pl, plan_lds, i);
-        pa_few_rows<HD, KVM, TERMS>(p, it, lds);
+    // workgroup 8 i + x goes to XCD x
+    const uint32_t half = PA_SHARES / 16, xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
+    const uint32_t k = gridDim.x < PA_SHARES ? blockIdx.x : (slot / half) * (PA_SHARES / 2) + xcd * half + slot % half;
+    unsigned long long w = k * pl.share;
+    const unsigned long long end = min(w + pl.share, pl.work);
+    while (w < end) {
+        const PaAt at = pa_find(p, pl, plan_lds, w);
+        const PaCut& c = at.c;
+        const uint32_t units = c.tiles * a.pool.nkv;
+        for (uint32_t u = at.unit; u < units && w < end; u++) {
+            const unsigned long long begin = at.w0 + (unsigned long long)u * c.unit, first = begin + p.cost.unit;  // the first block's place
+            // the blocks that begin in this share
+            const uint32_t i0 = w <= first ? 0u : ((uint32_t)(w - first) + c.block - 1) / c.block;
+            const uint32_t i1 = end >= begin + c.unit ? c.blocks : end <= first ? 0u : ((uint32_t)(end - first) + c.block - 1) / c.block;
+            if (i0 < i1) {
+                PaItem it;
+                it.x = at.x;
+                it.rows = c.rows;
+                it.kvh = u / c.tiles;
+                it.row0 = u % c.tiles * c.tile;
+                it.b0 = c.b0 + i0;
+                it.b1 = c.b0 + i1;
+                it.parts = at.x.parts || i0 != 0 || i1 != c.blocks;
+                it.part = (size_t)at.row0 + it.kvh * c.rows + it.row0 + (size_t)k * p.tile_many;
+                if (c.rows <= PA_FEW) {
+                    pa_few_rows<HD, KVM, TERMS>(p, it, reinterpret_cast<float*>(lds));
+                } else {
+                    float* const scales = reinterpret_cast<float*>(lds + pa_many_lds_halves<HD>() * 2);
+                    if (HD == 256 || c.rows - it.row0 <= 64) pa_many_rows<HD, KVM, TERMS, 1>(p, it, plan_lds, reinterpret_cast<_Float16*>(lds), scales);
+                    else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2>(p, it, plan_lds, reinterpret_cast<_Float16*>(lds), scales);
+                }
+            }
+            w = begin + c.unit;
+        }
     }
 }
 
 // ---------------------------------------------------------------------------
-// The parts of every row brought to a common maximum and added in order: the prefix' runs of keys, then the rest's.
-// HD / 4 lanes to a row.
+// The parts of every row brought to a common maximum and added in order: the prefix' parts, then the rest's.  HD / 4 lanes to a row.
 // ---------------------------------------------------------------------------
 template <int HD>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
@@ -577,6 +923,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
     constexpr uint32_t L = HD / 4, HPW = 256 / L;
     __shared__ uint32_t found;
     const uint32_t tid = threadIdx.x, c = tid % L, per_tok = (a.nq + HPW - 1) / HPW;
+    const unsigned long long share = p.entries[a.n_groups + a.n_requests].w0;
     for (uint64_t w = blockIdx.x; w < (uint64_t)a.n_tokens * per_tok; w += gridDim.x) {
         const uint32_t t = (uint32_t)(w / per_tok), h = (uint32_t)(w % per_tok) * HPW + tid / L;
         __syncthreads();
@@ -586,16 +933,32 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
             if (a.d_cu_tokens[r] <= (int)t && (int)t < a.d_cu_tokens[r + 1]) found = r;
         __syncthreads();
         const uint32_t r = found;
-        if (r == 0xFFFFFFFFu) continue;
-        const uint4 rest = p.entries[a.n_groups + r];
-        uint4 shared = make_uint4(0, 0, 0, 0);
-        if (a.n_groups) shared = p.entries[pa_group_of(a, r)];
-        if ((t - shared.w) * p.G >= shared.z) shared.y = 0;  // (a request of no group)
-        if (rest.y == 0 || h >= a.nq) continue;
+        if (r == 0xFFFFFFFFu || h >= a.nq) continue;
         const uint32_t kvh = h / p.G;
-        auto at = [&](const uint4& e, uint32_t i) -> size_t { return (size_t)e.x + ((size_t)i * a.pool.nkv + kvh) * e.z + (t - e.w) * p.G + h % p.G; };
-        const uint32_t n = shared.y + rest.y;
-        auto part = [&](uint32_t i) -> size_t { return i < shared.y ? at(shared, i) : at(rest, i - shared.y); };
+        // where this row's parts of an entry lie: `n` of them, tile_many rows apart
+        auto parts = [&](const PaLeft& e, uint32_t& n) -> size_t {
+            const uint32_t row = (t - e.t0) * p.G + h % p.G;
+            if (row >= e.rows) {  // (a request of no group)
+                n = 0;
+                return 0;
+            }
+            const unsigned long long first = e.w0 + (unsigned long long)(kvh * e.tiles + row / e.tile) * e.unit + p.cost.unit;
+            const uint32_t k0 = pa_div(first, share), k1 = pa_div(first + (unsigned long long)(e.blocks - 1) * e.block, share);
+            n = k1 - k0 + 1;
+            return (size_t)e.row0 + kvh * e.rows + row + (size_t)k0 * p.tile_many;
+        };
+        const PaLeft rest = p.entries[a.n_groups + r];
+        uint32_t n0 = 0, n1;
+        size_t p0 = 0;
+        if (rest.parts) {
+            const PaLeft shared = p.entries[pa_group_of(a, r)];
+            p0 = parts(shared, n0);
+        }
+        const size_t p1 = parts(rest, n1);
+        if (!rest.parts && n1 <= 1) continue;  // (written by the one that had it)
+        const uint32_t n = n0 + n1;
+        if (n == 0) continue;
+        auto part = [&](uint32_t i) -> size_t { return i < n0 ? p0 + (size_t)i * p.tile_many : p1 + (size_t)(i - n0) * p.tile_many; };
         float m = -INFINITY;
         for (uint32_t i0 = 0; i0 < n; i0 += 8) {
             float2 v[8];
@@ -629,17 +992,16 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
     }
 }
 
-// Parts at most: every row has one in its prefix and one in its rest; each further run of keys of an entry's tiles stands for
-// `each` blocks of work, of which there are PA_TARGET in all, and leaves PA_TILE rows.
-static uint64_t most_parts(const oxb_paged_attention& a) {
-    const uint64_t once = (uint64_t)a.n_tokens * a.nq;
-    return (a.n_groups ? 2 : 1) * once + (uint64_t)PA_TARGET * PA_TILE;
+// Rows of parts at most.  The part of unit u in share k begins u's rows and k tiles behind the first one: no two overlap, because the
+// next part is of the next unit or in the next share, and a tile has tile_many rows at most.
+static uint64_t most_rows(const oxb_paged_attention& a) {
+    return (uint64_t)a.n_tokens * a.nq * (a.n_groups ? 2 : 1) + (uint64_t)PA_SHARES * pa_tile_many(a.pool.hd);
 }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+static size_t entries_bytes(const oxb_paged_attention& a) { return up256(((size_t)a.n_groups + a.n_requests + 1) * sizeof(PaLeft)); }
 
 size_t oxb_paged_attention_workspace(const oxb_paged_attention& a) {
-    const uint64_t parts = most_parts(a);
-    return up256((size_t)(a.n_groups + a.n_requests) * sizeof(uint4)) + up256(parts * sizeof(float2)) + parts * a.pool.hd * sizeof(float);
+    return entries_bytes(a) + up256(most_rows(a) * sizeof(float2)) + most_rows(a) * a.pool.hd * sizeof(float);
 }
 
 template <int HD, int KVM>
@@ -650,16 +1012,11 @@ static void attention_launch(const PaParams& p, uint32_t grid, hipStream_t st) {
 template <int HD>
 static hipError_t attention_launch_hd(const PaParams& p, hipStream_t st) {
     const oxb_paged_attention& a = p.a;
-    // (no call can have more items than this: short ones start fewer workgroups)
-    const uint64_t keys = (uint64_t)a.table_width * a.pool.page_size, tiles = ((uint64_t)a.n_tokens * p.G + PA_TILE - 1) / PA_TILE;
-    const uint64_t items = ((a.n_groups ? 2 : 1) * tiles + a.n_requests + a.n_groups) * a.pool.nkv * ((keys + PA_BLOCK * PA_MIN_BLOCKS - 1) / (PA_BLOCK * PA_MIN_BLOCKS) + 1);
-    const uint32_t grid = (uint32_t)(items < PA_GRID ? items : PA_GRID);
-    if (a.pool.kv_dtype == OXB_KV_F16) attention_launch<HD, OXB_KV_F16>(p, grid, st);
-    else if (a.pool.kv_dtype == OXB_KV_I8) attention_launch<HD, OXB_KV_I8>(p, grid, st);
-    else attention_launch<HD, OXB_KV_FP8_E4M3>(p, grid, st);
-    hipError_t e = hipGetLastError();
-    // a table of so few keys is never split, and without prefixes every row is then written at once
-    if (e != hipSuccess || (a.n_groups == 0 && keys <= PA_BLOCK * PA_MIN_BLOCKS)) return e;
+    if (a.pool.kv_dtype == OXB_KV_F16) attention_launch<HD, OXB_KV_F16>(p, PA_SHARES, st);
+    else if (a.pool.kv_dtype == OXB_KV_I8) attention_launch<HD, OXB_KV_I8>(p, PA_SHARES, st);
+    else attention_launch<HD, OXB_KV_FP8_E4M3>(p, PA_SHARES, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
     const uint64_t wgs = (uint64_t)a.n_tokens * ((a.nq + 256 / (HD / 4) - 1) / (256 / (HD / 4)));
     hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3((uint32_t)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, st, p);
     return hipGetLastError();
@@ -669,13 +1026,17 @@ hipError_t oxb_launch_paged_attention(const oxb_paged_attention& a, hipStream_t 
     PaParams p;
     p.a = a;
     p.G = a.nq / a.pool.nkv;
-    p.scale_log2 = (a.scale == 0.f ? 1.0f / sqrtf((float)a.pool.hd) : a.scale) * PA_LOG2E;
+    p.scale_log2 = (a.scale == 0.f ? 1.0f / sqrtf((float)a.pool.hd) : fabsf(a.scale)) * PA_LOG2E;
+    p.negative = a.scale < 0.f ? 0x80000000u : 0u;
     p.page_shift = (uint32_t)__builtin_ctz(a.pool.page_size);
+    p.tile_many = pa_tile_many(a.pool.hd);
+    p.keys_many = pa_keys_many(a.pool.hd);
+    p.cost = a.pool.kv_dtype == OXB_KV_F16 ? PaCosts{12, 4, 8} : PaCosts{6, 5, 8};
     uint8_t* ws = reinterpret_cast<uint8_t*>(a.d_workspace);
-    p.entries = reinterpret_cast<uint4*>(ws);
-    ws += up256((size_t)(a.n_groups + a.n_requests) * sizeof(uint4));
+    p.entries = reinterpret_cast<PaLeft*>(ws);
+    ws += entries_bytes(a);
     p.ml = reinterpret_cast<float2*>(ws);
-    ws += up256(most_parts(a) * sizeof(float2));
+    ws += up256(most_rows(a) * sizeof(float2));
     p.o = reinterpret_cast<float*>(ws);
     switch (a.pool.hd) {
         case 32: return attention_launch_hd<32>(p, st);
