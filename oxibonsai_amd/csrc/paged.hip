@@ -59,6 +59,10 @@ int check_attention_counts(const oxb_paged_attention& a) {
     if (a.n_tokens == 0 || (uint64_t)a.n_tokens * a.nq > (1u << 30))
         return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: %u queries of %u heads (1 .. 2^30 rows)", a.n_tokens, a.nq);
     if (a.dtype > OXB_DTYPE_BF16) return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: type %u", a.dtype);
+    if (a.table_width == 0 || (uint64_t)a.table_width * a.pool.page_size > 0x7FFFFFFFu) return bad("table rows of no entries, or of 2^31 positions and more");
+    // the kernel counts the call's work in 32 bits: about a unit for 16 rows and 32 keys
+    const double tiles = (double)a.n_tokens * (a.nq / a.pool.nkv) / 16 + a.n_requests + a.n_groups, blocks = (double)a.table_width * a.pool.page_size / 32 + 10;
+    if ((a.n_groups ? 2 : 1) * tiles * a.pool.nkv * blocks >= 2147483648.0) return bad("more work than one call takes: too many queries over tables too wide");
     return OXB_HIP_OK;
 }
 
@@ -122,7 +126,6 @@ int oxb_hip_paged_attention_dev(const oxb_paged_attention* a) {
     if (!a) return bad("null descriptor");
     if (int rc = check_attention_counts(*a)) return rc;
     if (int rc = check_pool(a->pool)) return rc;
-    if (a->table_width == 0 || (uint64_t)a->table_width * a->pool.page_size > 0x7FFFFFFFu) return bad("table rows of no entries, or of 2^31 positions and more");
     const uint64_t wide = (uint64_t)a->nq * a->pool.hd;
     if (a->q_stride < wide || a->out_stride < wide || a->q_stride % 8 || a->out_stride % 8)
         return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: strides %u and %u (multiples of 8, at least %llu)", a->q_stride, a->out_stride, (unsigned long long)wide);

@@ -8,10 +8,11 @@
 // its products being all (query, q head) pairs of a kv head, and only the rests are read request by request.
 //
 // Work is cut on the device, because the lengths lie there.  An entry is a group's prefix or a request's rest, a unit one kv
-// head and tile of rows of an entry over all its keys, and the work of all units, laid end to end, is dealt out in equal shares, one
-// to a workgroup (512: two to a CU): every workgroup sums up the entries' work, finds where its share begins and walks from there,
-// the end of one unit, whole ones, the beginning of another.  A row whose unit lies in one share and has no other part is
-// written at once, other parts go to the workspace and a second launch adds them; there are at most 512 more parts than units.
+// head and tile of rows of an entry over all its keys.  The units' work, laid end to end, those of many rows first, is dealt out
+// in equal shares to 512 workgroups, two to a CU: every workgroup sums up the entries' work, finds where its share begins and
+// walks from there, the end of one unit, whole ones, the beginning of another.  Units of many rows are walked by a
+// workgroup, those of few rows by single waves, to each a quarter of the share.  A row whose unit lies in one share and has no other part
+// is written at once, other parts go to the workspace and a second launch adds them.
 // Workgroups go to the eight XCDs in turn; shares go to them in runs, so that what is read more than once (the prefix, by
 // each tile of rows of a kv head) is read at about the same time through one L2.  The first workgroup of a CU takes from the
 // first half, where the prefixes are, which are bound by the matrix cores, the second one from the second half, where the rests
@@ -29,19 +30,20 @@ typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 
 #define PA_SHARES 512u     // workgroups: two to a CU
-#define PA_FEW 32u         // rows up to which an entry's tiles have 16 rows and its waves take the keys in turn
+#define PA_FEW 32u         // rows up to which an entry's tiles have 16 rows and a wave to themselves
 #define PA_TILE_FEW 16u
-#define PA_KEYS_FEW 128u   // keys that a workgroup takes at a time: 32 by each wave
+#define PA_KEYS_FEW 32u    // keys that such a wave takes at a time
+#define PA_RUNS 256u       // runs of entries, one to a thread
 #define PA_LOG2E 1.44269504088896340736f
 
 // Tiles of many rows and the keys of a block of theirs: what the registers and two workgroups' LDS hold.
 constexpr uint32_t pa_tile_many(uint32_t hd) { return hd == 256 ? 64u : 128u; }
 constexpr uint32_t pa_keys_many(uint32_t hd) { return hd == 256 ? 32u : 64u; }
 
-// Work, in units that mean nothing but relative to each other: a block of keys for few rows (a wait for memory), for many rows
-// (products), and what a unit costs whatever its keys are.
+// Work, in units that mean nothing but relative to each other: a block of 32 keys for few rows, a block for many rows, and
+// what a unit of either costs whatever its keys are.
 struct PaCosts {
-    uint32_t few, many, unit;
+    uint32_t few, many, few_unit, many_unit;
 };
 
 struct PaParams {
@@ -52,7 +54,7 @@ struct PaParams {
     uint32_t page_shift;
     uint32_t tile_many, keys_many;
     PaCosts cost;
-    struct PaLeft* entries;  // workspace: what the merge needs of every entry; [n_groups + n_requests] is the share
+    struct PaLeft* entries;  // workspace: what the merge needs of every entry
     float2* ml;        // maximum (log2 units) and sum of every part's rows
     float* o;          // [rows of parts][hd]
 };
@@ -69,14 +71,15 @@ struct PaEntry {
 struct PaCut {
     uint32_t rows, tile, tiles;     // rows of a kv head, of a tile; tiles
     uint32_t keys, b0, blocks;      // keys of a block; the first block; how many
-    uint32_t block, unit;           // work of a block, of a unit
+    uint32_t block, fix, unit;      // work of a block, of a unit without its blocks, of a unit
+    bool few;
 };
 
 // What the attention leaves for the merge.
 struct PaLeft {
-    unsigned long long w0;          // where the entry's work begins
+    uint32_t w0;                    // where the entry's work begins
     uint32_t row0;                  // ... and its rows of parts
-    uint32_t rows, tile, tiles, blocks, block, unit, t0, parts, pad;
+    uint32_t rows, tile, tiles, blocks, block, fix, unit, t0, parts, per;  // per: work of a share of such units
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
@@ -128,124 +131,131 @@ __device__ __forceinline__ PaEntry pa_entry(const oxb_paged_attention& a, uint32
 __device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x) {
     PaCut c;
     c.rows = x.tn * p.G;
-    const bool few = c.rows <= PA_FEW;
-    c.tile = few ? PA_TILE_FEW : p.tile_many;
-    c.keys = few ? PA_KEYS_FEW : p.keys_many;
-    c.block = few ? p.cost.few : p.cost.many;
+    c.few = c.rows <= PA_FEW;
+    c.tile = c.few ? PA_TILE_FEW : p.tile_many;
+    c.keys = c.few ? PA_KEYS_FEW : p.keys_many;
+    c.block = c.few ? p.cost.few : p.cost.many;
+    c.fix = c.few ? p.cost.few_unit : p.cost.many_unit;
     c.tiles = (c.rows + c.tile - 1) / c.tile;
     c.b0 = x.k0 / c.keys;
     c.blocks = x.k1 > x.k0 ? (x.k1 + c.keys - 1) / c.keys - c.b0 : 1u;  // (a rest without keys is one block, in which nothing is seen)
-    c.unit = p.cost.unit + c.blocks * c.block;
+    c.unit = c.fix + c.blocks * c.block;
     return c;
 }
-// a / b; the numbers of nearly all calls have 32 bits
-__device__ __forceinline__ uint32_t pa_div(unsigned long long a, unsigned long long b) {
-    return (uint32_t)(((a | b) >> 32) == 0 ? (uint32_t)a / (uint32_t)b : a / b);
-}
 
-// What a workgroup knows about the whole call: its threads hold a run of entries each.
-struct PaPlan {
-    unsigned long long work, share;
-    uint32_t e0, e1;            // this thread's entries
-    unsigned long long w0;      // ... and where their work
-    uint32_t row0;              // ... and rows of parts begin
-};
-struct PaAt {                   // an entry in which a share has work
-    PaEntry x;
-    PaCut c;
-    unsigned long long w0;
-    uint32_t row0, unit;        // the unit in which the work begins
-};
+// The plan of a call, the same in every workgroup: thread i holds run i of the entries.
 struct PaPlanLds {
-    unsigned long long work[4];
-    uint32_t rows[4], bad[4], most[4];
-    PaAt at;
+    uint32_t work[2][4], rows[2][4], bad[4], most[4];
+    uint32_t w0[2][PA_RUNS], row0[2][PA_RUNS];  // where the work and the rows of parts of a run begin: those of many rows, those of few
+    PaEntry first[PA_RUNS];                     // a run's first entry
+};
+struct PaPlan {
+    uint32_t work, few0, share, per;   // all work, where that of few rows begins, a workgroup's share, entries to a run
 };
 
 __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, bool leave_entries) {
     const oxb_paged_attention& a = p.a;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_groups + a.n_requests, per = (E + 255u) / 256u;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_groups + a.n_requests;
     PaPlan pl;
-    pl.e0 = min(tid * per, E);
-    pl.e1 = min(pl.e0 + per, E);
-    unsigned long long work = 0;
-    uint32_t rows = 0;
+    pl.per = (E + PA_RUNS - 1) / PA_RUNS;
+    const uint32_t e0 = min(tid * pl.per, E), e1 = min(e0 + pl.per, E);
+    uint32_t work[2] = {0, 0}, rows[2] = {0, 0};
     bool bad = false;
-    for (uint32_t e = pl.e0; e < pl.e1; e++) {
+    for (uint32_t e = e0; e < e1; e++) {
         const PaEntry x = pa_entry(a, e);
         const PaCut c = pa_cut(p, x);
+        if (e == e0) lds.first[tid] = x;
         bad |= x.bad;
-        work += (unsigned long long)c.unit * c.tiles * a.pool.nkv;
-        rows += c.rows * a.pool.nkv;
+        work[c.few] += c.unit * c.tiles * a.pool.nkv;
+        rows[c.few] += c.rows * a.pool.nkv;
     }
-    unsigned long long iw = work;
-    uint32_t ir = rows;
+    uint32_t iw[2] = {work[0], work[1]}, ir[2] = {rows[0], rows[1]};
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const unsigned long long ow = __shfl_up(iw, d, 64);
-        const uint32_t orr = __shfl_up(ir, d, 64);
-        if (lane >= (uint32_t)d) iw += ow, ir += orr;
-    }
+    for (int d = 1; d < 64; d *= 2)
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            const uint32_t ow = __shfl_up(iw[f], d, 64), orr = __shfl_up(ir[f], d, 64);
+            if (lane >= (uint32_t)d) iw[f] += ow, ir[f] += orr;
+        }
     bad = __builtin_amdgcn_ballot_w64(bad) != 0;
-    if (lane == 63) lds.work[wave] = iw, lds.rows[wave] = ir, lds.bad[wave] = bad;
+    if (lane == 63) {
+#pragma unroll
+        for (int f = 0; f < 2; f++) lds.work[f][wave] = iw[f], lds.rows[f][wave] = ir[f];
+        lds.bad[wave] = bad;
+    }
     __syncthreads();
-    pl.w0 = iw - work;
-    pl.row0 = ir - rows;
-    pl.work = 0;
+    uint32_t w0[2] = {iw[0] - work[0], iw[1] - work[1]}, row0[2] = {ir[0] - rows[0], ir[1] - rows[1]}, all[2] = {0, 0}, all_rows = 0;
     bad = false;
+#pragma unroll
     for (uint32_t w = 0; w < 4; w++) {
-        if (w < wave) pl.w0 += lds.work[w], pl.row0 += lds.rows[w];
-        pl.work += lds.work[w];
+#pragma unroll
+        for (int f = 0; f < 2; f++) {
+            if (w < wave) w0[f] += lds.work[f][w], row0[f] += lds.rows[f][w];
+            all[f] += lds.work[f][w];
+        }
+        all_rows += lds.rows[0][w];
         bad |= lds.bad[w] != 0;
     }
-    // (no share without a block: parts are counted by the blocks that begin in a share)
-    pl.share = max((pl.work + PA_SHARES - 1) / PA_SHARES, (unsigned long long)max(p.cost.few, p.cost.many));
+    pl.few0 = uniform(all[0]);
+    pl.work = uniform(all[0] + all[1]);
+    w0[1] += all[0];
+    row0[1] += all_rows + PA_SHARES * p.tile_many;
+#pragma unroll
+    for (int f = 0; f < 2; f++) lds.w0[f][tid] = w0[f], lds.row0[f][tid] = row0[f];
+    // four waves to a share, and no share without a block: parts are counted by the blocks that begin in a share
+    pl.share = max(((pl.work + PA_SHARES - 1) / PA_SHARES + 3) & ~3u, max(4 * p.cost.few, p.cost.many));
     // (with sums that do not ascend the parts could pass the workspace: nothing is done at all)
     if (bad) pl.work = 0;
     if (leave_entries) {
-        unsigned long long w = pl.w0;
-        uint32_t row = pl.row0;
-        for (uint32_t e = pl.e0; e < pl.e1; e++) {
+        for (uint32_t e = e0; e < e1; e++) {
             const PaEntry x = pa_entry(a, e);
             const PaCut c = pa_cut(p, x);
-            p.entries[e] = {w, row, bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.block, c.unit, x.t0, x.parts, 0};
-            w += (unsigned long long)c.unit * c.tiles * a.pool.nkv;
-            row += c.rows * a.pool.nkv;
+            const int f = c.few;
+            p.entries[e] = {w0[f], row0[f], bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.block, c.fix, c.unit, x.t0, x.parts, f ? pl.share / 4 : pl.share};
+            w0[f] += c.unit * c.tiles * a.pool.nkv;
+            row0[f] += c.rows * a.pool.nkv;
         }
-        if (tid == 0) p.entries[E].w0 = pl.share;
     }
+    __syncthreads();
     return pl;
 }
 
-// The entry in which the work at w lies, found by the thread that holds it and left in LDS for all (two barriers).
-__device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, PaPlanLds& lds, unsigned long long w) {
+// The entry of many (few 0) or few rows in which the work at w lies: every wave for itself.  w lies in front of the end of that
+// kind's work, so the last run that begins at or in front of w, of those that have any, holds it.
+struct PaAt {
+    PaEntry x;
+    PaCut c;
+    uint32_t w0, row0;
+};
+__device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, const PaPlanLds& lds, uint32_t few, uint32_t w) {
     const oxb_paged_attention& a = p.a;
-    unsigned long long at = pl.w0;
-    uint32_t row = pl.row0;
-    __syncthreads();
-    if (w >= at)
-        for (uint32_t e = pl.e0; e < pl.e1; e++) {
-            const PaEntry x = pa_entry(a, e);
-            const PaCut c = pa_cut(p, x);
-            const unsigned long long n = (unsigned long long)c.unit * c.tiles * a.pool.nkv;
-            if (w - at < n) {
-                lds.at = {x, c, at, row, pa_div(w - at, c.unit)};
-                break;
-            }
-            at += n;
-            row += c.rows * a.pool.nkv;
-        }
-    __syncthreads();
-    PaAt r = lds.at;  // the same for all: into scalar registers
-    r.x.t0 = uniform(r.x.t0), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1), r.x.table = uniform(r.x.table), r.x.parts = uniform(r.x.parts) != 0;
-    r.c.rows = uniform(r.c.rows), r.c.tile = uniform(r.c.tile), r.c.tiles = uniform(r.c.tiles), r.c.b0 = uniform(r.c.b0);
-    r.c.blocks = uniform(r.c.blocks), r.c.block = uniform(r.c.block), r.c.unit = uniform(r.c.unit), r.c.keys = uniform(r.c.keys);
-    r.row0 = uniform(r.row0), r.unit = uniform(r.unit);
-    r.w0 = (unsigned long long)uniform((uint32_t)(r.w0 >> 32)) << 32 | uniform((uint32_t)r.w0);
+    const uint32_t lane = threadIdx.x & 63u, E = a.n_groups + a.n_requests;
+    uint32_t run = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < PA_RUNS / 64; i++) run += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(lds.w0[few][i * 64 + lane] <= w));
+    run -= 1;
+    uint32_t e = run * pl.per;
+    PaAt r;
+    r.x = lds.first[run];
+    r.w0 = lds.w0[few][run];
+    r.row0 = lds.row0[few][run];
+    for (;;) {
+        r.c = pa_cut(p, r.x);
+        const uint32_t n = r.c.few == (few != 0) ? r.c.unit * r.c.tiles * a.pool.nkv : 0u;
+        if (w - r.w0 < n || ++e >= E) break;
+        r.w0 += n;
+        r.row0 += n ? r.c.rows * a.pool.nkv : 0u;
+        r.x = pa_entry(a, e);
+    }
+    // the same for the whole wave: into scalar registers
+    r.x.t0 = uniform(r.x.t0), r.x.tn = uniform(r.x.tn), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1), r.x.table = uniform(r.x.table);
+    r.x.parts = uniform(r.x.parts) != 0;
+    r.c = pa_cut(p, r.x);
+    r.w0 = uniform(r.w0), r.row0 = uniform(r.row0);
     return r;
 }
 
-// What a workgroup does at a time: blocks b0 .. b1 of a tile of an entry's rows.
+// What is done at a time: blocks b0 .. b1 of a tile of an entry's rows.
 struct PaItem {
     PaEntry x;
     uint32_t rows, row0, kvh;  // rows of a kv head; the tile's first
@@ -253,6 +263,34 @@ struct PaItem {
     size_t part;               // where the tile's rows of parts begin
     bool parts;
 };
+// The items of a share [w, end) of one kind of work, one after the other; k: the share's number among those of its size.
+template <typename F>
+__device__ __forceinline__ void pa_walk(const PaParams& p, const PaPlan& pl, const PaPlanLds& lds, uint32_t few, uint32_t w, uint32_t end, uint32_t k, F item) {
+    while (w < end) {
+        const PaAt at = pa_find(p, pl, lds, few, w);
+        const PaCut& c = at.c;
+        const uint32_t units = c.tiles * p.a.pool.nkv;
+        for (uint32_t u = (w - at.w0) / c.unit; u < units && w < end; u++) {
+            const uint32_t begin = at.w0 + u * c.unit, first = begin + c.fix;  // the first block's place
+            // the blocks that begin in this share
+            const uint32_t i0 = w <= first ? 0u : (w - first + c.block - 1) / c.block;
+            const uint32_t i1 = end >= begin + c.unit ? c.blocks : end <= first ? 0u : (end - first + c.block - 1) / c.block;
+            if (i0 < i1) {
+                PaItem it;
+                it.x = at.x;
+                it.rows = c.rows;
+                it.kvh = u / c.tiles;
+                it.row0 = u % c.tiles * c.tile;
+                it.b0 = c.b0 + i0;
+                it.b1 = c.b0 + i1;
+                it.parts = at.x.parts || i0 != 0 || i1 != c.blocks;
+                it.part = (size_t)at.row0 + it.kvh * c.rows + it.row0 + (size_t)k * c.tile;
+                item(it);
+            }
+            w = begin + c.unit;
+        }
+    }
+}
 
 // Eight values of q from memory, as fp32, times the scale's sign.
 __device__ __forceinline__ void pa_load_q8(const void* q, uint32_t dtype, uint32_t sign, size_t at, float v[8]) {
@@ -288,8 +326,8 @@ __device__ __forceinline__ void pa_store4(void* out, uint32_t dtype, size_t at, 
 __device__ __forceinline__ float pa_lse(float m, float l) { return l > 0.f ? (m + log2f(l)) * 0.693147180559945309417f : l == 0.f ? -INFINITY : NAN; }
 
 // ---------------------------------------------------------------------------
-// Few rows: a request's rest, a small group's prefix.  16 rows, the four waves take 32 keys each of a block of 128 and add their
-// sums in LDS at the end; operands come from memory straight into registers, the next block's while this one is worked on.
+// Few rows: a request's rest, a small group's prefix.  A wave has 16 rows and shares nothing with the others; operands come from
+// memory straight into registers, the next block of 32 keys while this one is worked on.
 //
 // Products as in the prefill attention, transposed, on v_mfma_f32_16x16x32_f16: S^T = K Q^T leaves a lane (row c = lane % 16,
 // g = lane / 16) the scores of keys 4 g .. and 16 + 4 g .. of a block, which is where O^T = V^T P^T wants its probabilities.  V as
@@ -330,31 +368,59 @@ __device__ __forceinline__ void pa_read(uint32_t (&d)[N], const uint8_t* p) {
 }
 
 template <int HD, int KVM, int TERMS>
-__device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it, float* lds) {
+__device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it) {
     typedef PaBlock<HD, KVM> Block;
     constexpr bool QC = Block::QC;
     constexpr int KS = Block::KS, DPL = Block::DPL;
     constexpr uint32_t ROWB = HD * (QC ? 1 : 2);
     const oxb_paged_attention& a = p.a;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
-    const uint32_t wave = uniform(tid >> 6);
+    const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, g = lane >> 4;
+    const uint32_t lo = it.x.k0, kvh = it.kvh;
+
+    const int32_t* const table_row = a.d_tables + (size_t)it.x.table * a.table_width;
+    typedef const __attribute__((address_space(4))) int32_t* ConstInts;  // (nothing writes the tables meanwhile: scalar loads)
+    const ConstInts table = (ConstInts)(uintptr_t)table_row;
+    const uint8_t* const Kc = reinterpret_cast<const uint8_t*>(a.pool.d_k);
+    const uint8_t* const Vc = reinterpret_cast<const uint8_t*>(a.pool.d_v);
+    const uint32_t last = it.x.k1 - 1;  // (only used where there are keys)
+    // First row of the 16 positions from `at` on, which lie in one page.
+    auto row_of = [&](uint32_t at) -> size_t {
+        const uint32_t page = (uint32_t)table[at >> p.page_shift], safe = min(page, a.pool.n_pages - 1);
+        return (((size_t)kvh * a.pool.n_pages + safe) << p.page_shift) + (at & (a.pool.page_size - 1u));
+    };
+    auto request = [&](Block& B, uint32_t b) {
+#pragma unroll
+        for (uint32_t kt = 0; kt < 2; kt++) {
+            // rows in front of the entry's first key or behind its last one are not read: they need hold no numbers
+            const uint32_t at = max(min(b * 32u + 16 * kt, last & ~15u), lo & ~15u), to = min(last - at, 15u), from = min(lo > at ? lo - at : 0u, to);
+            const size_t r = row_of(at);
+            const uint8_t *kr = Kc + r * ROWB, *vr = Vc + r * ROWB;
+            const uint32_t kc = max(min(c, to), from) * ROWB;
+#pragma unroll
+            for (int s = 0; s < Block::KW; s++) pa_read(B.k[kt][s], kr + kc + (QC ? (KS > 1 ? 64u * s + 16u * g : 8u * g) : 64u * s + 16u * g));
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint8_t* vp = vr + max(min(4 * g + e, to), from) * ROWB + c * (DPL * (QC ? 1 : 2));
+                if constexpr (DPL * (QC ? 1 : 2) >= 4) pa_read(B.v[4 * kt + e], vp);
+                else B.v[4 * kt + e][0] = *reinterpret_cast<const uint16_t*>(vp);
+            }
+            if constexpr (QC) {
+                B.ks[kt] = *reinterpret_cast<const v4f*>(a.pool.d_k_scale + r + 4 * g);
+                B.vs[kt] = *reinterpret_cast<const v4f*>(a.pool.d_v_scale + r + 4 * g);
+            }
+        }
+    };
+    // (two blocks of wide rows do not fit the registers)
+    constexpr bool AHEAD = HD < 256;
+    const bool any = it.x.k1 > lo;
+    Block A, B;
+    if (any) request(A, it.b0);
+
     // this lane's row
     const uint32_t row = it.row0 + c;
     const bool there = row < it.rows;
     const uint32_t tok = it.x.t0 + (there ? row : it.rows - 1) / p.G, head = it.kvh * p.G + (there ? row : it.rows - 1) % p.G;
     const int pos = a.d_positions[tok];
-    const uint32_t sees = min(pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), it.x.k1);  // keys in front of this one
-    uint32_t most = there ? sees : 0u, least = there ? sees : 0xFFFFFFFFu;
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-        most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
-        least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
-    }
-    most = uniform(most);
-    least = uniform(least);
-    const uint32_t lo = it.x.k0, kvh = it.kvh;
-    const uint32_t b1 = most > lo ? min(4 * it.b1, (most + 31u) / 32u) : 0u;  // (nothing is seen behind)
-
     // q: element e of step s is dimension dim(s) + e
     auto dim = [&](int s) -> uint32_t { return QC && KS > 1 ? 64u * (s / 2) + 16u * g + 8u * (s % 2) : 32u * s + 8u * g; };
     v8h q[TERMS][KS];
@@ -381,39 +447,16 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
             }
     }
 
-    typedef const __attribute__((address_space(4))) int32_t* ConstInts;  // (nothing writes the tables meanwhile: scalar loads)
-    const ConstInts table = (ConstInts)(uintptr_t)(a.d_tables + (size_t)it.x.table * a.table_width);
-    const uint8_t* const Kc = reinterpret_cast<const uint8_t*>(a.pool.d_k);
-    const uint8_t* const Vc = reinterpret_cast<const uint8_t*>(a.pool.d_v);
-    const uint32_t last = most - 1;  // (only used where something is seen)
-    // First row of the 16 positions from `at` on, which lie in one page.
-    auto row_of = [&](uint32_t at) -> size_t {
-        const uint32_t page = (uint32_t)table[at >> p.page_shift], safe = min(page, a.pool.n_pages - 1);
-        return (((size_t)kvh * a.pool.n_pages + safe) << p.page_shift) + (at & (a.pool.page_size - 1u));
-    };
-    auto request = [&](Block& B, uint32_t b) {
+    const uint32_t sees = min(pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), it.x.k1);  // keys in front of this one
+    uint32_t most = there ? sees : 0u, least = there ? sees : 0xFFFFFFFFu;
 #pragma unroll
-        for (uint32_t kt = 0; kt < 2; kt++) {
-            // rows in front of the first key or behind the last one that is seen are not read: they need hold no numbers
-            const uint32_t at = max(min(b * 32u + 16 * kt, last & ~15u), lo & ~15u), from = lo > at ? min(lo - at, 15u) : 0u, to = min(last - at, 15u);
-            const size_t r = row_of(at);
-            const uint8_t *kr = Kc + r * ROWB, *vr = Vc + r * ROWB;
-            const uint32_t kc = max(min(c, to), min(from, to)) * ROWB;
-#pragma unroll
-            for (int s = 0; s < Block::KW; s++) pa_read(B.k[kt][s], kr + kc + (QC ? (KS > 1 ? 64u * s + 16u * g : 8u * g) : 64u * s + 16u * g));
-#pragma unroll
-            for (uint32_t e = 0; e < 4; e++) {
-                const uint8_t* vp = vr + max(min(4 * g + e, to), min(from, to)) * ROWB + c * (DPL * (QC ? 1 : 2));
-                if constexpr (DPL * (QC ? 1 : 2) >= 4) pa_read(B.v[4 * kt + e], vp);
-                else B.v[4 * kt + e][0] = *reinterpret_cast<const uint16_t*>(vp);
-            }
-            if constexpr (QC) {
-                B.ks[kt] = *reinterpret_cast<const v4f*>(a.pool.d_k_scale + r + 4 * g);
-                B.vs[kt] = *reinterpret_cast<const v4f*>(a.pool.d_v_scale + r + 4 * g);
-            }
-        }
-    };
-
+    for (int d = 1; d < 16; d *= 2) {
+        most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+        least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
+    }
+    most = uniform(most);
+    least = uniform(least);
+    const uint32_t b1 = any ? min(it.b1, (most + 31u) / 32u) : 0u;  // (nothing is seen behind)
     v4f O[DPL];
 #pragma unroll
     for (int j = 0; j < DPL; j++) O[j] = (v4f){0.f, 0.f, 0.f, 0.f};
@@ -507,70 +550,45 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it,
             for (int t = 0; t < TERMS; t++) O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V, P[t], O[j], 0, 0, 0);
         }
     };
-    // (two blocks of wide rows do not fit the registers)
-    constexpr bool AHEAD = HD < 256;
-    const uint32_t b0 = 4 * it.b0 + wave;
     if constexpr (AHEAD) {
-        Block A, B;
-        if (b0 < b1) request(A, b0);
-        for (uint32_t b = b0; b < b1; b += 8) {
-            if (b + 4 < b1) request(B, b + 4);
+        for (uint32_t b = it.b0; b < b1; b += 2) {
+            if (b + 1 < b1) request(B, b + 1);
             block(A, b);
-            if (b + 4 >= b1) break;
-            if (b + 8 < b1) request(A, b + 8);
-            block(B, b + 4);
+            if (b + 1 >= b1) break;
+            if (b + 2 < b1) request(A, b + 2);
+            block(B, b + 1);
         }
     } else {
-        for (uint32_t b = b0; b < b1; b += 4) {
-            Block A;
-            request(A, b);
+        for (uint32_t b = it.b0; b < b1; b++) {
+            if (b > it.b0) request(A, b);
             block(A, b);
         }
     }
     l = sum_rows4(l);
-
-    // the four waves' sums
-    constexpr uint32_t LD = HD + 4;  // (floats of a row in LDS)
-    float* const lo_o = lds;                                      // [4][16][LD]
-    float2* const lo_ml = reinterpret_cast<float2*>(lds + 4 * 16 * LD);  // [4][16]
-    __syncthreads();
-    if (g == 0) lo_ml[wave * 16 + c] = make_float2(m, l);
+    if (!there) return;
+    const size_t part = it.part + c;
+    const float inv = it.parts ? 1.f : l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-    for (int v = 0; v < 4; v++)
+    for (int v = 0; v < 4; v++) {
+        float o[DPL < 4 ? 4 : DPL];
 #pragma unroll
-        for (int j = 0; j < DPL; j++) lo_o[(wave * 16 + c) * LD + (4 * g + v) * DPL + j] = O[j][v];
-    __syncthreads();
-    // row r of the tile by 16 threads, HD / 16 dimensions each: four at a time, 64 apart
-    const uint32_t r = tid >> 4, u = tid & 15u, out_row = it.row0 + r;
-    if (out_row >= it.rows) return;
-    float2 w[4];
-    float top = -INFINITY, sum = 0.f, f[4];
+        for (int j = 0; j < DPL; j++) o[j] = O[j][v] * inv;
+        const uint32_t d = (4 * g + v) * DPL;
+        if constexpr (DPL >= 4) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) w[i] = lo_ml[i * 16 + r], top = w[i].x > top ? w[i].x : top;
-    const float ref = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int i = 0; i < 4; i++) f[i] = __builtin_amdgcn_exp2f(w[i].x - ref), sum = fmaf(w[i].y, f[i], sum);
-    const uint32_t t = it.x.t0 + out_row / p.G, h = it.kvh * p.G + out_row % p.G;
-    const size_t part = it.part + r;
-    const float inv = it.parts ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
-    constexpr uint32_t STEP = HD < 64 ? HD : 64;
-    if (4 * u < STEP)
-#pragma unroll
-        for (uint32_t d = 4 * u; d < HD; d += STEP) {
-            float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4 x = *reinterpret_cast<const float4*>(lo_o + (i * 16 + r) * LD + d);
-                o[0] = fmaf(x.x, f[i], o[0]), o[1] = fmaf(x.y, f[i], o[1]), o[2] = fmaf(x.z, f[i], o[2]), o[3] = fmaf(x.w, f[i], o[3]);
+            for (int j = 0; j < DPL; j += 4) {
+                if (it.parts) *reinterpret_cast<float4*>(p.o + part * HD + d + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                else pa_store4(a.d_out, a.dtype, (size_t)tok * a.out_stride + (size_t)head * HD + d + j, o + j);
             }
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[i] *= inv;
-            if (it.parts) *reinterpret_cast<float4*>(p.o + part * HD + d) = make_float4(o[0], o[1], o[2], o[3]);
-            else pa_store4(a.d_out, a.dtype, (size_t)t * a.out_stride + (size_t)h * HD + d, o);
+        } else {
+            if (it.parts) *reinterpret_cast<float2*>(p.o + part * HD + d) = make_float2(o[0], o[1]);
+            else if (a.dtype == OXB_DTYPE_F32) *reinterpret_cast<float2*>(reinterpret_cast<float*>(a.d_out) + (size_t)tok * a.out_stride + (size_t)head * HD + d) = make_float2(o[0], o[1]);
+            else *reinterpret_cast<uint32_t*>(reinterpret_cast<uint16_t*>(a.d_out) + (size_t)tok * a.out_stride + (size_t)head * HD + d) = pa_bits16(o[0], a.dtype) | pa_bits16(o[1], a.dtype) << 16;
         }
-    if (u == 0) {
-        if (it.parts) p.ml[part] = make_float2(top, sum);
-        else if (a.d_lse) a.d_lse[(size_t)t * a.nq + h] = pa_lse(top, sum);
+    }
+    if (g == 0) {
+        if (it.parts) p.ml[part] = make_float2(m, l);
+        else if (a.d_lse) a.d_lse[(size_t)tok * a.nq + head] = pa_lse(m, l);
     }
 }
 
@@ -603,64 +621,12 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
     const uint32_t wave = uniform(tid >> 6);
     const uint32_t lo = it.x.k0, kvh = it.kvh;
 
-    uint32_t tok[QT], head[QT], sees[QT], most = 0, least = 0xFFFFFFFFu;
-    bool there[QT];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        const uint32_t row = it.row0 + (t * 4 + wave) * 16 + c, r = min(row, it.rows - 1);
-        there[t] = row < it.rows;
-        tok[t] = it.x.t0 + r / p.G;
-        head[t] = kvh * p.G + r % p.G;
-        const int pos = a.d_positions[tok[t]];
-        sees[t] = min(pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), it.x.k1);
-        most = max(most, there[t] ? sees[t] : 0u);
-        least = min(least, there[t] ? sees[t] : 0xFFFFFFFFu);
-    }
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-        most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
-        least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
-    }
-    most = uniform(most);
-    least = uniform(least);
-    __syncthreads();
-    if (lane == 0) plan_lds.most[wave] = most;
-    __syncthreads();
-    const uint32_t wg_most = uniform(max(max(plan_lds.most[0], plan_lds.most[1]), max(plan_lds.most[2], plan_lds.most[3])));
-    const uint32_t last = wg_most - 1;
-    const uint32_t b1 = wg_most > lo ? min(it.b1, last / KB + 1) : 0u;
-
-    // q as in the other form; element e of step s is dimension 32 s + 8 g + e
-    v8h q[TERMS][QT][KS];
-    float mul[QT];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-        float f[KS][8], top = 0.f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            pa_load_q8(a.d_q, a.dtype, p.negative, (size_t)tok[t] * a.q_stride + (size_t)head[t] * HD + 32 * s + 8 * g, f[s]);
-#pragma unroll
-            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[s][e]));
-        }
-        top = max_rows4(top);
-        const int ex = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-        mul[t] = __builtin_amdgcn_ldexpf(p.scale_log2, ex);
-#pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float x = __builtin_amdgcn_ldexpf(f[s][e], -ex);
-                const _Float16 hi = (_Float16)x;
-                q[0][t][s][e] = hi;
-                if constexpr (TERMS == 2) q[1][t][s][e] = (_Float16)(x - (float)hi);
-            }
-    }
-
     typedef const __attribute__((address_space(4))) int32_t* ConstInts;
     const ConstInts table = (ConstInts)(uintptr_t)(a.d_tables + (size_t)it.x.table * a.table_width);
     const uint8_t* const Kc = reinterpret_cast<const uint8_t*>(a.pool.d_k);
     const uint8_t* const Vc = reinterpret_cast<const uint8_t*>(a.pool.d_v);
     _Float16 *const ks0 = lds, *const vs0 = lds + KB * HD, *const ks1 = lds + 2 * KB * HD, *const vs1 = lds + 3 * KB * HD;
+    const uint32_t last = it.x.k1 - 1;  // (only used where there are keys)
     // this wave's rows of block b: positions `at` .. in one page; those in front of the first key or behind the last one are not read
     auto rows_of = [&](uint32_t b, uint32_t& from, uint32_t& to) -> size_t {
         const uint32_t at = max(min(b * KB + wave * RPW, last & ~(uint32_t)(RPW - 1)), lo & ~(uint32_t)(RPW - 1));
@@ -724,6 +690,57 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
 
+    const bool any = it.x.k1 > lo;
+    __syncthreads();  // (the item before has been read)
+    if (any) request(it.b0, ks0, vs0);
+
+    uint32_t tok[QT], head[QT], sees[QT], most = 0, least = 0xFFFFFFFFu;
+    bool there[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const uint32_t row = it.row0 + (t * 4 + wave) * 16 + c, r = min(row, it.rows - 1);
+        there[t] = row < it.rows;
+        tok[t] = it.x.t0 + r / p.G;
+        head[t] = kvh * p.G + r % p.G;
+        const int pos = a.d_positions[tok[t]];
+        sees[t] = min(pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), it.x.k1);
+        most = max(most, there[t] ? sees[t] : 0u);
+        least = min(least, there[t] ? sees[t] : 0xFFFFFFFFu);
+    }
+#pragma unroll
+    for (int d = 1; d < 16; d *= 2) {
+        most = max(most, (uint32_t)__shfl_xor((int)most, d, 64));
+        least = min(least, (uint32_t)__shfl_xor((int)least, d, 64));
+    }
+    most = uniform(most);
+    least = uniform(least);
+
+    // q as in the other form; element e of step s is dimension 32 s + 8 g + e
+    v8h q[TERMS][QT][KS];
+    float mul[QT];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        float f[KS][8], top = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            pa_load_q8(a.d_q, a.dtype, p.negative, (size_t)tok[t] * a.q_stride + (size_t)head[t] * HD + 32 * s + 8 * g, f[s]);
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[s][e]));
+        }
+        top = max_rows4(top);
+        const int ex = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
+        mul[t] = __builtin_amdgcn_ldexpf(p.scale_log2, ex);
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float x = __builtin_amdgcn_ldexpf(f[s][e], -ex);
+                const _Float16 hi = (_Float16)x;
+                q[0][t][s][e] = hi;
+                if constexpr (TERMS == 2) q[1][t][s][e] = (_Float16)(x - (float)hi);
+            }
+    }
+
     // K operand of step 0 in the first 16 keys, V operand of the first 16 dimensions in the first 16 keys (halves); step s and
     // dimension tile sl are an XOR away
     const uint32_t k_at = (c * PPR + (g ^ ((c / RB) & PM))) * 8;
@@ -740,25 +757,49 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
     auto block = [&](const _Float16* kb, const _Float16* vb, const float* sc, uint32_t b) {
         const uint32_t key0 = b * KB;
         if (key0 >= most) return;  // (wave-uniform) nothing for this wave's rows
+        // Operands are requested ahead of their use, and the fences hold the compiler to that order: K of the next 32 keys right after
+        // its registers' last use, V in groups of VB, the first of them while the probabilities are worked out.
+        auto fence = [&]() { __builtin_amdgcn_sched_barrier(0); };
+        constexpr int NP = NH * NS, VB = NP < 4 ? NP : TERMS == 2 || QC ? 2 : 4;
+        v8h K[2][KS], V[2][VB];
+        auto read_k = [&](int hb, int s) {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) K[kt][s] = *reinterpret_cast<const v8h*>(kb + (k_at ^ (32u * s)) + (2 * hb + kt) * 16 * HD);
+        };
+        auto read_v = [&](int j) {
+#pragma unroll
+            for (int u = 0; u < VB; u++) {
+                const int i = j * VB + u;
+                const _Float16* tile = vb + (v_at ^ (16u * (i % NS))) + (i / NS) * 32 * HD;
+                const v4h_t t0 = lds_read_tr16(tile), t1 = lds_read_tr16(tile + 16 * HD);
+                V[j & 1][u] = (v8h){t0[0], t0[1], t0[2], t0[3], t1[0], t1[1], t1[2], t1[3]};
+            }
+        };
         v4f S[QT][NT];
 #pragma unroll
-        for (int hb = 0; hb < NH; hb++) {
-            v8h K[2][KS];
+        for (int s = 0; s < KS; s++) read_k(0, s);
+        fence();
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+        for (int t = 0; t < QT; t++)
 #pragma unroll
-                for (int kt = 0; kt < 2; kt++) K[kt][s] = *reinterpret_cast<const v8h*>(kb + (k_at ^ (32u * s)) + (2 * hb + kt) * 16 * HD);
+            for (int kt = 0; kt < NT; kt++) S[t][kt] = (v4f){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int t = 0; t < QT; t++) S[t][2 * hb] = S[t][2 * hb + 1] = (v4f){0.f, 0.f, 0.f, 0.f};
+        for (int hb = 0; hb < NH; hb++)
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int s = 0; s < KS; s++) {
 #pragma unroll
                 for (int n = 0; n < TERMS; n++)
 #pragma unroll
                     for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                         for (int t = 0; t < QT; t++) S[t][2 * hb + kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K[kt][s], q[n][t][s], S[t][2 * hb + kt], 0, 0, 0);
-        }
+                if (hb + 1 < NH) {
+                    read_k(hb + 1, s);
+                    fence();
+                }
+            }
+        read_v(0);
+        fence();
         const bool all = key0 >= lo && key0 + KB <= least;  // (wave-uniform) every row sees all of these keys
         v8h P[TERMS][QT][NH];
         float vs[NT][4];
@@ -824,23 +865,28 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             l[t] += sum;
         }
 #pragma unroll
-        for (int hb = 0; hb < NH; hb++)
+        for (int j = 0; j < NP / VB; j++) {
+            if (j + 1 < NP / VB) read_v(j + 1);
+            fence();
 #pragma unroll
-            for (int i = 0; i < NS; i++) {
-                const _Float16* tile = vb + (v_at ^ (16u * i)) + hb * 32 * HD;
-                const v4h_t t0 = lds_read_tr16(tile), t1 = lds_read_tr16(tile + 16 * HD);
-                const v8h V = {t0[0], t0[1], t0[2], t0[3], t1[0], t1[1], t1[2], t1[3]};
+            for (int u = 0; u < VB; u++)
 #pragma unroll
                 for (int n = 0; n < TERMS; n++)
 #pragma unroll
-                    for (int t = 0; t < QT; t++) O[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V, P[n][t][hb], O[t][i], 0, 0, 0);
-            }
+                    for (int t = 0; t < QT; t++) {
+                        const int i = j * VB + u;
+                        O[t][i % NS] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V[j & 1][u], P[n][t][i / NS], O[t][i % NS], 0, 0, 0);
+                    }
+        }
     };
     float *const sc0 = scales, *const sc1 = scales + 2 * KB;
-    if (it.b0 < b1) {
-        request(it.b0, ks0, vs0);
+    if (any) {
+        if (lane == 0) plan_lds.most[wave] = most;
         deliver(ks0, vs0, sc0, true);
-        for (uint32_t b = it.b0;;) {
+        // nothing is seen behind the last query's keys
+        const uint32_t wg_most = uniform(max(max(plan_lds.most[0], plan_lds.most[1]), max(plan_lds.most[2], plan_lds.most[3])));
+        const uint32_t b1 = min(it.b1, (wg_most + KB - 1) / KB);
+        for (uint32_t b = it.b0; b < b1;) {
             if (b + 1 < b1) request(b + 1, ks1, vs1);
             block(ks0, vs0, sc0, b);
             if (++b >= b1) break;
@@ -872,46 +918,20 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 
 template <int HD, int KVM, int TERMS>
 __global__ __launch_bounds__(256, 2) void paged_attention_kernel(PaParams p) {
-    constexpr int FEW = (4 * 16 * (HD + 4) + 4 * 16 * 2) * 4, MANY = pa_many_lds_halves<HD>() * 2 + 4 * (int)pa_keys_many(HD) * 4;
     __shared__ PaPlanLds plan_lds;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[FEW > MANY ? FEW : MANY];
-    const oxb_paged_attention& a = p.a;
+    __shared__ __attribute__((aligned(16))) _Float16 lds[pa_many_lds_halves<HD>()];
+    __shared__ __attribute__((aligned(16))) float scales[4 * pa_keys_many(HD)];
     const PaPlan pl = pa_plan(p, plan_lds, blockIdx.x == 0);
     // workgroup 8 i + x goes to XCD x
     const uint32_t half = PA_SHARES / 16, xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
-    const uint32_t k = gridDim.x < PA_SHARES ? blockIdx.x : (slot / half) * (PA_SHARES / 2) + xcd * half + slot % half;
-    unsigned long long w = k * pl.share;
-    const unsigned long long end = min(w + pl.share, pl.work);
-    while (w < end) {
-        const PaAt at = pa_find(p, pl, plan_lds, w);
-        const PaCut& c = at.c;
-        const uint32_t units = c.tiles * a.pool.nkv;
-        for (uint32_t u = at.unit; u < units && w < end; u++) {
-            const unsigned long long begin = at.w0 + (unsigned long long)u * c.unit, first = begin + p.cost.unit;  // the first block's place
-            // the blocks that begin in this share
-            const uint32_t i0 = w <= first ? 0u : ((uint32_t)(w - first) + c.block - 1) / c.block;
-            const uint32_t i1 = end >= begin + c.unit ? c.blocks : end <= first ? 0u : ((uint32_t)(end - first) + c.block - 1) / c.block;
-            if (i0 < i1) {
-                PaItem it;
-                it.x = at.x;
-                it.rows = c.rows;
-                it.kvh = u / c.tiles;
-                it.row0 = u % c.tiles * c.tile;
-                it.b0 = c.b0 + i0;
-                it.b1 = c.b0 + i1;
-                it.parts = at.x.parts || i0 != 0 || i1 != c.blocks;
-                it.part = (size_t)at.row0 + it.kvh * c.rows + it.row0 + (size_t)k * p.tile_many;
-                if (c.rows <= PA_FEW) {
-                    pa_few_rows<HD, KVM, TERMS>(p, it, reinterpret_cast<float*>(lds));
-                } else {
-                    float* const scales = reinterpret_cast<float*>(lds + pa_many_lds_halves<HD>() * 2);
-                    if (HD == 256 || c.rows - it.row0 <= 64) pa_many_rows<HD, KVM, TERMS, 1>(p, it, plan_lds, reinterpret_cast<_Float16*>(lds), scales);
-                    else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2>(p, it, plan_lds, reinterpret_cast<_Float16*>(lds), scales);
-                }
-            }
-            w = begin + c.unit;
-        }
-    }
+    const uint32_t k = (slot / half) * (PA_SHARES / 2) + xcd * half + slot % half;
+    const uint32_t w = k < pl.work / pl.share + 1 ? k * pl.share : pl.work, end = min(w + pl.share, pl.work);
+    pa_walk(p, pl, plan_lds, 0, w, min(end, pl.few0), k, [&](const PaItem& it) {
+        if (HD == 256 || it.rows - it.row0 <= 64) pa_many_rows<HD, KVM, TERMS, 1>(p, it, plan_lds, lds, scales);
+        else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2>(p, it, plan_lds, lds, scales);
+    });
+    const uint32_t wave = uniform(threadIdx.x >> 6), quarter = pl.share / 4, from = w + wave * quarter;
+    pa_walk(p, pl, plan_lds, 1, max(from, pl.few0), min(from + quarter, end), 4 * k + wave, [&](const PaItem& it) { pa_few_rows<HD, KVM, TERMS>(p, it); });
 }
 
 // ---------------------------------------------------------------------------
@@ -923,7 +943,6 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
     constexpr uint32_t L = HD / 4, HPW = 256 / L;
     __shared__ uint32_t found;
     const uint32_t tid = threadIdx.x, c = tid % L, per_tok = (a.nq + HPW - 1) / HPW;
-    const unsigned long long share = p.entries[a.n_groups + a.n_requests].w0;
     for (uint64_t w = blockIdx.x; w < (uint64_t)a.n_tokens * per_tok; w += gridDim.x) {
         const uint32_t t = (uint32_t)(w / per_tok), h = (uint32_t)(w % per_tok) * HPW + tid / L;
         __syncthreads();
@@ -935,30 +954,30 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
         const uint32_t r = found;
         if (r == 0xFFFFFFFFu || h >= a.nq) continue;
         const uint32_t kvh = h / p.G;
-        // where this row's parts of an entry lie: `n` of them, tile_many rows apart
+        // where this row's parts of an entry lie: `n` of them, a tile apart
         auto parts = [&](const PaLeft& e, uint32_t& n) -> size_t {
             const uint32_t row = (t - e.t0) * p.G + h % p.G;
             if (row >= e.rows) {  // (a request of no group)
                 n = 0;
                 return 0;
             }
-            const unsigned long long first = e.w0 + (unsigned long long)(kvh * e.tiles + row / e.tile) * e.unit + p.cost.unit;
-            const uint32_t k0 = pa_div(first, share), k1 = pa_div(first + (unsigned long long)(e.blocks - 1) * e.block, share);
-            n = k1 - k0 + 1;
-            return (size_t)e.row0 + kvh * e.rows + row + (size_t)k0 * p.tile_many;
+            const uint32_t first = e.w0 + (kvh * e.tiles + row / e.tile) * e.unit + e.fix, k0 = first / e.per;
+            n = (first + (e.blocks - 1) * e.block) / e.per - k0 + 1;
+            return (size_t)e.row0 + kvh * e.rows + row + (size_t)k0 * e.tile;
         };
         const PaLeft rest = p.entries[a.n_groups + r];
-        uint32_t n0 = 0, n1;
+        uint32_t n0 = 0, n1, tile0 = 0;
         size_t p0 = 0;
         if (rest.parts) {
             const PaLeft shared = p.entries[pa_group_of(a, r)];
             p0 = parts(shared, n0);
+            tile0 = shared.tile;
         }
         const size_t p1 = parts(rest, n1);
         if (!rest.parts && n1 <= 1) continue;  // (written by the one that had it)
         const uint32_t n = n0 + n1;
         if (n == 0) continue;
-        auto part = [&](uint32_t i) -> size_t { return i < n0 ? p0 + (size_t)i * p.tile_many : p1 + (size_t)(i - n0) * p.tile_many; };
+        auto part = [&](uint32_t i) -> size_t { return i < n0 ? p0 + (size_t)i * tile0 : p1 + (size_t)(i - n0) * rest.tile; };
         float m = -INFINITY;
         for (uint32_t i0 = 0; i0 < n; i0 += 8) {
             float2 v[8];
@@ -992,13 +1011,13 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
     }
 }
 
-// Rows of parts at most.  The part of unit u in share k begins u's rows and k tiles behind the first one: no two overlap, because the
-// next part is of the next unit or in the next share, and a tile has tile_many rows at most.
+// Rows of parts at most.  The part of unit u in share k begins u's rows and k tiles behind the first one of its kind: no two overlap,
+// because the next part is of the next unit or in the next share, and no unit has more rows than a tile.
 static uint64_t most_rows(const oxb_paged_attention& a) {
-    return (uint64_t)a.n_tokens * a.nq * (a.n_groups ? 2 : 1) + (uint64_t)PA_SHARES * pa_tile_many(a.pool.hd);
+    return (uint64_t)a.n_tokens * a.nq * (a.n_groups ? 2 : 1) + (uint64_t)PA_SHARES * (pa_tile_many(a.pool.hd) + 4 * PA_TILE_FEW);
 }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
-static size_t entries_bytes(const oxb_paged_attention& a) { return up256(((size_t)a.n_groups + a.n_requests + 1) * sizeof(PaLeft)); }
+static size_t entries_bytes(const oxb_paged_attention& a) { return up256(((size_t)a.n_groups + a.n_requests) * sizeof(PaLeft)); }
 
 size_t oxb_paged_attention_workspace(const oxb_paged_attention& a) {
     return entries_bytes(a) + up256(most_rows(a) * sizeof(float2)) + most_rows(a) * a.pool.hd * sizeof(float);
@@ -1031,7 +1050,7 @@ hipError_t oxb_launch_paged_attention(const oxb_paged_attention& a, hipStream_t 
     p.page_shift = (uint32_t)__builtin_ctz(a.pool.page_size);
     p.tile_many = pa_tile_many(a.pool.hd);
     p.keys_many = pa_keys_many(a.pool.hd);
-    p.cost = a.pool.kv_dtype == OXB_KV_F16 ? PaCosts{12, 4, 8} : PaCosts{6, 5, 8};
+    p.cost = a.pool.kv_dtype == OXB_KV_F16 ? PaCosts{1, 2, 2, 4} : PaCosts{1, 4, 2, 8};
     uint8_t* ws = reinterpret_cast<uint8_t*>(a.d_workspace);
     p.entries = reinterpret_cast<PaLeft*>(ws);
     ws += entries_bytes(a);
