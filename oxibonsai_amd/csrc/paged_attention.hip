@@ -7,16 +7,17 @@
 // sum_parts exp(m_part - m) (l_part, o_part) is the whole.  So the prefix is read once for all queries of the group, the rows of
 // its products being all (query, q head) pairs of a kv head, and only the rests are read request by request.
 //
-// Work is cut on the device, because the lengths lie there.  An entry is a group's prefix or a request's rest, a unit one kv
-// head and tile of rows of an entry over all its keys.  The units' work, laid end to end, those of many rows first, is dealt out
-// in equal shares to 512 workgroups, two to a CU: every workgroup sums up the entries' work, finds where its share begins and
-// walks from there, the end of one unit, whole ones, the beginning of another.  Units of many rows are walked by a
-// workgroup, those of few rows by single waves, to each a quarter of the share.  A row whose unit lies in one share and has no other part
-// is written at once, other parts go to the workspace and a second launch adds them.
-// Workgroups go to the eight XCDs in turn; shares go to them in runs, so that what is read more than once (the prefix, by
-// each tile of rows of a kv head) is read at about the same time through one L2.  The first workgroup of a CU takes from the
-// first half, where the prefixes are, which are bound by the matrix cores, the second one from the second half, where the rests
-// are, which are bound by memory.
+// Work is cut on the device, because the lengths lie there.  An entry is a group's prefix or a request's rest, a unit one tile of
+// its rows of a kv head over a segment of its keys (all of them where the rows are few).  The units' work, laid end to end, those
+// of many rows first, is dealt out in equal shares to 512 workgroups, two to a CU: every workgroup sums up the entries'
+// work, finds where its share begins and walks from there, the end of one unit, whole ones, the beginning of another.  Units of
+// many rows are walked by a workgroup, those of few rows by single waves, to each a quarter of the share.  A row whose keys
+// lie in one unit and share is written at once, other parts go to the workspace and a second launch adds them.
+// Workgroups go to the eight XCDs in turn, shares go to them in runs; a segment is about a share long and the tiles of its
+// rows follow each other, so they walk the same keys at the same time and meet in one L2 (whole walks per tile instead:
+// 2.9 us for 64 keys of 128 rows where that takes 1.2, 256 requests behind 16000 keys, every tile's keys from memory).
+// The first workgroup of a CU takes from the first half, where the prefixes are, which are bound by the matrix cores, the second
+// one from the second half, where the rests are, which are bound by memory.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -38,7 +39,7 @@ typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 
 // Tiles of many rows and the keys of a block of theirs: what the registers and two workgroups' LDS hold.
 constexpr uint32_t pa_tile_many(uint32_t hd) { return hd == 256 ? 64u : 128u; }
-constexpr uint32_t pa_keys_many(uint32_t hd) { return hd == 256 ? 32u : 64u; }
+constexpr uint32_t pa_keys_many(uint32_t hd, bool one_byte, bool two_terms) { return hd == 256 || one_byte || two_terms ? 32u : 64u; }
 
 // Work, in units that mean nothing but relative to each other: a block of 32 keys for few rows, a block for many rows, and
 // what a unit of either costs whatever its keys are.
@@ -71,7 +72,9 @@ struct PaEntry {
 struct PaCut {
     uint32_t rows, tile, tiles;     // rows of a kv head, of a tile; tiles
     uint32_t keys, b0, blocks;      // keys of a block; the first block; how many
+    uint32_t segs, seg;             // segments; blocks of one, the last one may have fewer
     uint32_t block, fix, unit;      // work of a block, of a unit without its blocks, of a unit
+    uint32_t units;
     bool few;
 };
 
@@ -79,7 +82,7 @@ struct PaCut {
 struct PaLeft {
     uint32_t w0;                    // where the entry's work begins
     uint32_t row0;                  // ... and its rows of parts
-    uint32_t rows, tile, tiles, blocks, block, fix, unit, t0, parts, per;  // per: work of a share of such units
+    uint32_t rows, tile, tiles, blocks, segs, seg, block, fix, unit, t0, parts, per, few, pad;  // per: work of a share of such units
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
@@ -128,7 +131,8 @@ __device__ __forceinline__ PaEntry pa_entry(const oxb_paged_attention& a, uint32
     x.tn = t1 > x.t0 ? t1 - x.t0 : 0u;
     return x;
 }
-__device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x) {
+// `length`: work of a segment at most.
+__device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x, uint32_t length) {
     PaCut c;
     c.rows = x.tn * p.G;
     c.few = c.rows <= PA_FEW;
@@ -139,18 +143,23 @@ __device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x) {
     c.tiles = (c.rows + c.tile - 1) / c.tile;
     c.b0 = x.k0 / c.keys;
     c.blocks = x.k1 > x.k0 ? (x.k1 + c.keys - 1) / c.keys - c.b0 : 1u;  // (a rest without keys is one block, in which nothing is seen)
-    c.unit = c.fix + c.blocks * c.block;
+    c.segs = c.few ? 1u : (c.blocks * c.block + length - 1) / length;
+    c.seg = (c.blocks + c.segs - 1) / c.segs;
+    c.segs = (c.blocks + c.seg - 1) / c.seg;
+    c.unit = c.fix + c.seg * c.block;
+    c.units = c.tiles * c.segs * p.a.pool.nkv;
     return c;
 }
 
 // The plan of a call, the same in every workgroup: thread i holds run i of the entries.
 struct PaPlanLds {
-    uint32_t work[2][4], rows[2][4], bad[4], most[4];
+    uint32_t sum[4], work[2][4], rows[2][4], bad[4], most[4];
     uint32_t w0[2][PA_RUNS], row0[2][PA_RUNS];  // where the work and the rows of parts of a run begin: those of many rows, those of few
     PaEntry first[PA_RUNS];                     // a run's first entry
 };
 struct PaPlan {
     uint32_t work, few0, share, per;   // all work, where that of few rows begins, a workgroup's share, entries to a run
+    uint32_t length;                   // work of a segment, at most
 };
 
 __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, bool leave_entries) {
@@ -159,15 +168,27 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     PaPlan pl;
     pl.per = (E + PA_RUNS - 1) / PA_RUNS;
     const uint32_t e0 = min(tid * pl.per, E), e1 = min(e0 + pl.per, E);
-    uint32_t work[2] = {0, 0}, rows[2] = {0, 0};
+    // the work as it were if every unit had all its keys gives the length of a segment
+    uint32_t whole = 0;
     bool bad = false;
+    PaEntry first;
     for (uint32_t e = e0; e < e1; e++) {
         const PaEntry x = pa_entry(a, e);
-        const PaCut c = pa_cut(p, x);
-        if (e == e0) lds.first[tid] = x;
+        const PaCut c = pa_cut(p, x, 0xFFFFFFFFu);
+        if (e == e0) lds.first[tid] = first = x;
         bad |= x.bad;
-        work[c.few] += c.unit * c.tiles * a.pool.nkv;
-        rows[c.few] += c.rows * a.pool.nkv;
+        whole += c.unit * c.units;
+    }
+#pragma unroll
+    for (int d = 32; d; d /= 2) whole += __shfl_xor(whole, d, 64);
+    if (lane == 0) lds.sum[wave] = whole;
+    __syncthreads();
+    pl.length = uniform(max((lds.sum[0] + lds.sum[1] + lds.sum[2] + lds.sum[3] + PA_SHARES - 1) / PA_SHARES, p.cost.many));
+    uint32_t work[2] = {0, 0}, rows[2] = {0, 0};
+    for (uint32_t e = e0; e < e1; e++) {
+        const PaCut c = pa_cut(p, e == e0 ? first : pa_entry(a, e), pl.length);
+        work[c.few] += c.unit * c.units;
+        rows[c.few] += c.rows * c.segs * a.pool.nkv;
     }
     uint32_t iw[2] = {work[0], work[1]}, ir[2] = {rows[0], rows[1]};
 #pragma unroll
@@ -199,7 +220,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     pl.few0 = uniform(all[0]);
     pl.work = uniform(all[0] + all[1]);
     w0[1] += all[0];
-    row0[1] += all_rows + PA_SHARES * p.tile_many;
+    row0[1] += all_rows + PA_SHARES * p.tile_many;  // (behind the parts of many rows)
 #pragma unroll
     for (int f = 0; f < 2; f++) lds.w0[f][tid] = w0[f], lds.row0[f][tid] = row0[f];
     // four waves to a share, and no share without a block: parts are counted by the blocks that begin in a share
@@ -209,11 +230,11 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     if (leave_entries) {
         for (uint32_t e = e0; e < e1; e++) {
             const PaEntry x = pa_entry(a, e);
-            const PaCut c = pa_cut(p, x);
+            const PaCut c = pa_cut(p, x, pl.length);
             const int f = c.few;
-            p.entries[e] = {w0[f], row0[f], bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.block, c.fix, c.unit, x.t0, x.parts, f ? pl.share / 4 : pl.share};
-            w0[f] += c.unit * c.tiles * a.pool.nkv;
-            row0[f] += c.rows * a.pool.nkv;
+            p.entries[e] = {w0[f], row0[f], bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.segs, c.seg, c.block, c.fix, c.unit, x.t0, x.parts, f ? pl.share / 4 : pl.share, c.few, 0};
+            w0[f] += c.unit * c.units;
+            row0[f] += c.rows * c.segs * a.pool.nkv;
         }
     }
     __syncthreads();
@@ -240,17 +261,17 @@ __device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, con
     r.w0 = lds.w0[few][run];
     r.row0 = lds.row0[few][run];
     for (;;) {
-        r.c = pa_cut(p, r.x);
-        const uint32_t n = r.c.few == (few != 0) ? r.c.unit * r.c.tiles * a.pool.nkv : 0u;
+        r.c = pa_cut(p, r.x, pl.length);
+        const uint32_t n = r.c.few == (few != 0) ? r.c.unit * r.c.units : 0u;
         if (w - r.w0 < n || ++e >= E) break;
         r.w0 += n;
-        r.row0 += n ? r.c.rows * a.pool.nkv : 0u;
+        r.row0 += n ? r.c.rows * r.c.segs * a.pool.nkv : 0u;
         r.x = pa_entry(a, e);
     }
     // the same for the whole wave: into scalar registers
     r.x.t0 = uniform(r.x.t0), r.x.tn = uniform(r.x.tn), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1), r.x.table = uniform(r.x.table);
     r.x.parts = uniform(r.x.parts) != 0;
-    r.c = pa_cut(p, r.x);
+    r.c = pa_cut(p, r.x, pl.length);
     r.w0 = uniform(r.w0), r.row0 = uniform(r.row0);
     return r;
 }
@@ -269,22 +290,22 @@ __device__ __forceinline__ void pa_walk(const PaParams& p, const PaPlan& pl, con
     while (w < end) {
         const PaAt at = pa_find(p, pl, lds, few, w);
         const PaCut& c = at.c;
-        const uint32_t units = c.tiles * p.a.pool.nkv;
-        for (uint32_t u = (w - at.w0) / c.unit; u < units && w < end; u++) {
+        for (uint32_t u = (w - at.w0) / c.unit; u < c.units && w < end; u++) {
             const uint32_t begin = at.w0 + u * c.unit, first = begin + c.fix;  // the first block's place
+            const uint32_t tile = u % c.tiles, seg = u / c.tiles % c.segs, n = min(c.seg, c.blocks - seg * c.seg);
             // the blocks that begin in this share
             const uint32_t i0 = w <= first ? 0u : (w - first + c.block - 1) / c.block;
-            const uint32_t i1 = end >= begin + c.unit ? c.blocks : end <= first ? 0u : (end - first + c.block - 1) / c.block;
+            const uint32_t i1 = min(n, end >= begin + c.unit ? n : end <= first ? 0u : (end - first + c.block - 1) / c.block);
             if (i0 < i1) {
                 PaItem it;
                 it.x = at.x;
                 it.rows = c.rows;
-                it.kvh = u / c.tiles;
-                it.row0 = u % c.tiles * c.tile;
-                it.b0 = c.b0 + i0;
-                it.b1 = c.b0 + i1;
-                it.parts = at.x.parts || i0 != 0 || i1 != c.blocks;
-                it.part = (size_t)at.row0 + it.kvh * c.rows + it.row0 + (size_t)k * c.tile;
+                it.kvh = u / c.tiles / c.segs;
+                it.row0 = tile * c.tile;
+                it.b0 = c.b0 + seg * c.seg + i0;
+                it.b1 = c.b0 + seg * c.seg + i1;
+                it.parts = at.x.parts || c.segs > 1 || i0 != 0 || i1 != n;
+                it.part = (size_t)at.row0 + (size_t)(u / c.tiles) * c.rows + it.row0 + (size_t)k * c.tile;
                 item(it);
             }
             w = begin + c.unit;
@@ -602,38 +623,42 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
 // reads (two tiles share an operand) and the VALU's softmax about equally: 512 cycles each per 32 keys of head_dim 128 and
 // wave.
 // ---------------------------------------------------------------------------
-template <int HD>
-constexpr int pa_many_lds_halves() {
-    return 4 * (int)pa_keys_many(HD) * HD;
-}
+// K and V of two blocks: arrays of their own, so that the compiler sees that a read of one need not wait for what is on its way
+// to another.
+struct PaStages {
+    _Float16 *k0, *v0, *k1, *v1;
+    float* scales;
+};
 
 template <int HD, int KVM, int TERMS, int QT>
-__device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it, PaPlanLds& plan_lds, _Float16* lds, float* scales) {
+__device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it, PaPlanLds& plan_lds, const PaStages& st) {
     constexpr bool QC = KVM != OXB_KV_F16;
-    constexpr int KB = (int)pa_keys_many(HD), KS = HD / 32, NS = HD / 16, NT = KB / 16, NH = KB / 32;
+    constexpr int KB = (int)pa_keys_many(HD, KVM != OXB_KV_F16, TERMS == 2), KS = HD / 32, NS = HD / 16, NT = KB / 16, NH = KB / 32;
     constexpr uint32_t ROWB = HD * (QC ? 1 : 2);
     constexpr int PPR = HD / 8, RPW = KB / 4;                       // pieces of an LDS row; rows that a wave fetches
     constexpr int RB = PPR >= 16 ? 1 : 16 / PPR, PM = (PPR < 16 ? PPR : 16) - 1;  // rows of 256 bytes; the permutation's mask
     constexpr int NI = (RPW * (int)ROWB / 16 + 63) / 64;            // 16-byte pieces per lane and block, of K and of V
-    constexpr bool HALF = RPW * ROWB / 16 < 64;                     // half a wave holds them all
+    constexpr bool HALF = RPW * ROWB / 16 < 64;                     // a part of a wave holds them all
     const oxb_paged_attention& a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
     const uint32_t wave = uniform(tid >> 6);
     const uint32_t lo = it.x.k0, kvh = it.kvh;
 
-    typedef const __attribute__((address_space(4))) int32_t* ConstInts;
-    const ConstInts table = (ConstInts)(uintptr_t)(a.d_tables + (size_t)it.x.table * a.table_width);
+    const int32_t* const table = a.d_tables + (size_t)it.x.table * a.table_width;
     const uint8_t* const Kc = reinterpret_cast<const uint8_t*>(a.pool.d_k);
     const uint8_t* const Vc = reinterpret_cast<const uint8_t*>(a.pool.d_v);
-    _Float16 *const ks0 = lds, *const vs0 = lds + KB * HD, *const ks1 = lds + 2 * KB * HD, *const vs1 = lds + 3 * KB * HD;
+    _Float16 *const ks0 = st.k0, *const vs0 = st.v0, *const ks1 = st.k1, *const vs1 = st.v1;
     const uint32_t last = it.x.k1 - 1;  // (only used where there are keys)
     // this wave's rows of block b: positions `at` .. in one page; those in front of the first key or behind the last one are not read
+    auto at_of = [&](uint32_t b) -> uint32_t { return max(min(b * KB + wave * RPW, last & ~(uint32_t)(RPW - 1)), lo & ~(uint32_t)(RPW - 1)); };
+    // The page of the next request travels with the rows of the one before.
+    auto page_of = [&](uint32_t b) -> uint32_t { return (uint32_t)table[at_of(b) >> p.page_shift]; };
+    uint32_t page = 0;
     auto rows_of = [&](uint32_t b, uint32_t& from, uint32_t& to) -> size_t {
-        const uint32_t at = max(min(b * KB + wave * RPW, last & ~(uint32_t)(RPW - 1)), lo & ~(uint32_t)(RPW - 1));
+        const uint32_t at = at_of(b);
         to = min(last - at, (uint32_t)RPW - 1);
         from = min(lo > at ? lo - at : 0u, to);
-        const uint32_t page = (uint32_t)table[at >> p.page_shift], safe = min(page, a.pool.n_pages - 1);
-        return (((size_t)kvh * a.pool.n_pages + safe) << p.page_shift) + (at & (a.pool.page_size - 1u));
+        return (((size_t)kvh * a.pool.n_pages + min(uniform(page), a.pool.n_pages - 1)) << p.page_shift) + (at & (a.pool.page_size - 1u));
     };
     v4w kreg[QC ? NI : 1], vreg[QC ? NI : 1];
     float kscale = 0.f, vscale = 0.f;
@@ -646,11 +671,10 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             constexpr uint32_t SPR = ROWB / 16;  // pieces of a cache row
             const uint32_t id = i * 64 + lane, r = id / SPR, piece = QC ? id % SPR : (id % SPR) ^ (((wave * RPW + r) / RB) & PM);
             const uint32_t off = max(min(r, to), from) * ROWB + piece * 16;
+            if (HALF && lane >= RPW * ROWB / 16) continue;
             if constexpr (QC) {
-                if (!HALF || lane < RPW * ROWB / 16) {
-                    kreg[i] = *reinterpret_cast<const v4w*>(kb + off);
-                    vreg[i] = *reinterpret_cast<const v4w*>(vb + off);
-                }
+                kreg[i] = *reinterpret_cast<const v4w*>(kb + off);
+                vreg[i] = *reinterpret_cast<const v4w*>(vb + off);
             } else {
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + off),
                                                  (__attribute__((address_space(3))) void*)(kd + (wave * RPW * PPR + i * 64) * 8), 16, 0, 0);
@@ -663,6 +687,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             kscale = a.pool.d_k_scale[row + r];
             vscale = a.pool.d_v_scale[row + r];
         }
+        page = page_of(b + 1);
     };
     // The barrier that ends a block: every wave has read it, and the next one is complete in LDS.
     auto deliver = [&](_Float16* kd, _Float16* vd, float* sc, bool there_is) {
@@ -692,7 +717,10 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 
     const bool any = it.x.k1 > lo;
     __syncthreads();  // (the item before has been read)
-    if (any) request(it.b0, ks0, vs0);
+    if (any) {
+        page = page_of(it.b0);
+        request(it.b0, ks0, vs0);
+    }
 
     uint32_t tok[QT], head[QT], sees[QT], most = 0, least = 0xFFFFFFFFu;
     bool there[QT];
@@ -816,29 +844,40 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
                 }
             }
         }
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-            if (!all) {
-#pragma unroll
-                for (int kt = 0; kt < NT; kt++)
-#pragma unroll
-                    for (int v = 0; v < 4; v++) {
-                        const uint32_t key = key0 + 16 * kt + 4 * g + v;
-                        S[t][kt][v] = key >= lo && key < sees[t] ? S[t][kt][v] : -INFINITY;
-                    }
-            }
-            float top = -INFINITY;
+        if (!all) {
 #pragma unroll
             for (int kt = 0; kt < NT; kt++)
 #pragma unroll
                 for (int v = 0; v < 4; v++) {
-                    if constexpr (QC) top = fmaxf(top, fmaf(S[t][kt][v], mul[t], (float)((int)(max(__float_as_uint(vs[kt][v]) & 0x7FFFFFFFu, 27u << 23) >> 23) - 127)));
-                    else top = fmaxf(top, S[t][kt][v]);
+                    const uint32_t key = key0 + 16 * kt + 4 * g + v;
+#pragma unroll
+                    for (int t = 0; t < QT; t++) S[t][kt][v] = key >= lo && key < sees[t] ? S[t][kt][v] : -INFINITY;
                 }
-            top = max_rows4(top);
-            if constexpr (!QC) top *= mul[t];
-            if (__builtin_amdgcn_ballot_w64(top > m[t])) {
-                const float now = fmaxf(top, m[t]), by = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
+        }
+        // (the tiles side by side: one's latencies are the other's work)
+        float top[QT], ref[QT], sum[QT][2];
+        bool more = false;
+#pragma unroll
+        for (int t = 0; t < QT; t++) top[t] = -INFINITY;
+#pragma unroll
+        for (int kt = 0; kt < NT; kt++)
+#pragma unroll
+            for (int v = 0; v < 4; v++) {
+                float e = 0.f;
+                if constexpr (QC) e = (float)((int)(max(__float_as_uint(vs[kt][v]) & 0x7FFFFFFFu, 27u << 23) >> 23) - 127);
+#pragma unroll
+                for (int t = 0; t < QT; t++) top[t] = fmaxf(top[t], QC ? fmaf(S[t][kt][v], mul[t], e) : S[t][kt][v]);
+            }
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            top[t] = max_rows4(top[t]);
+            if constexpr (!QC) top[t] *= mul[t];
+            more |= top[t] > m[t];
+        }
+        if (__builtin_amdgcn_ballot_w64(more)) {
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                const float now = fmaxf(top[t], m[t]), by = m[t] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[t] - now);
                 m[t] = now;
                 l[t] *= by;
 #pragma unroll
@@ -846,14 +885,28 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 #pragma unroll
                     for (int v = 0; v < 4; v++) O[t][i][v] *= by;
             }
-            const float ref = m[t] == -INFINITY ? 0.f : m[t];
-            float sum = 0.f;
+        }
 #pragma unroll
-            for (int kt = 0; kt < NT; kt++)
+        for (int t = 0; t < QT; t++) {
+            ref[t] = m[t] == -INFINITY ? 0.f : m[t];
+            sum[t][0] = sum[t][1] = 0.f;
+        }
 #pragma unroll
-                for (int v = 0; v < 4; v++) {
-                    float x = __builtin_amdgcn_exp2f(fmaf(S[t][kt][v], mul[t], -ref));
-                    sum += x;
+        for (int kt = 0; kt < NT; kt++) {
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int t = 0; t < QT; t++) S[t][kt][v] = fmaf(S[t][kt][v], mul[t], -ref[t]);
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int t = 0; t < QT; t++) S[t][kt][v] = __builtin_amdgcn_exp2f(S[t][kt][v]);
+#pragma unroll
+            for (int v = 0; v < 4; v++)
+#pragma unroll
+                for (int t = 0; t < QT; t++) {
+                    float x = S[t][kt][v];
+                    sum[t][v & 1] += x;
                     if constexpr (QC) {
                         x *= vs[kt][v];
                         if constexpr (TERMS == 2) asm("" : "+v"(x));  // (see above)
@@ -862,8 +915,9 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
                     P[0][t][kt / 2][4 * (kt % 2) + v] = hi;
                     if constexpr (TERMS == 2) P[1][t][kt / 2][4 * (kt % 2) + v] = (_Float16)(x - (float)hi);
                 }
-            l[t] += sum;
         }
+#pragma unroll
+        for (int t = 0; t < QT; t++) l[t] += sum[t][0] + sum[t][1];
 #pragma unroll
         for (int j = 0; j < NP / VB; j++) {
             if (j + 1 < NP / VB) read_v(j + 1);
@@ -879,7 +933,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
                     }
         }
     };
-    float *const sc0 = scales, *const sc1 = scales + 2 * KB;
+    float *const sc0 = st.scales, *const sc1 = st.scales + 2 * KB;
     if (any) {
         if (lane == 0) plan_lds.most[wave] = most;
         deliver(ks0, vs0, sc0, true);
@@ -917,18 +971,20 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 }
 
 template <int HD, int KVM, int TERMS>
-__global__ __launch_bounds__(256, 2) void paged_attention_kernel(PaParams p) {
+__global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel(PaParams p) {
     __shared__ PaPlanLds plan_lds;
-    __shared__ __attribute__((aligned(16))) _Float16 lds[pa_many_lds_halves<HD>()];
-    __shared__ __attribute__((aligned(16))) float scales[4 * pa_keys_many(HD)];
+    constexpr int KB = (int)pa_keys_many(HD, KVM != OXB_KV_F16, TERMS == 2);
+    __shared__ __attribute__((aligned(16))) _Float16 k0[KB * HD], v0[KB * HD], k1[KB * HD], v1[KB * HD];
+    __shared__ __attribute__((aligned(16))) float scales[4 * KB];
+    const PaStages st = {k0, v0, k1, v1, scales};
     const PaPlan pl = pa_plan(p, plan_lds, blockIdx.x == 0);
     // workgroup 8 i + x goes to XCD x
     const uint32_t half = PA_SHARES / 16, xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
     const uint32_t k = (slot / half) * (PA_SHARES / 2) + xcd * half + slot % half;
     const uint32_t w = k < pl.work / pl.share + 1 ? k * pl.share : pl.work, end = min(w + pl.share, pl.work);
     pa_walk(p, pl, plan_lds, 0, w, min(end, pl.few0), k, [&](const PaItem& it) {
-        if (HD == 256 || it.rows - it.row0 <= 64) pa_many_rows<HD, KVM, TERMS, 1>(p, it, plan_lds, lds, scales);
-        else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2>(p, it, plan_lds, lds, scales);
+        if (HD == 256 || it.rows - it.row0 <= 64) pa_many_rows<HD, KVM, TERMS, 1>(p, it, plan_lds, st);
+        else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2>(p, it, plan_lds, st);
     });
     const uint32_t wave = uniform(threadIdx.x >> 6), quarter = pl.share / 4, from = w + wave * quarter;
     pa_walk(p, pl, plan_lds, 1, max(from, pl.few0), min(from + quarter, end), 4 * k + wave, [&](const PaItem& it) { pa_few_rows<HD, KVM, TERMS>(p, it); });
@@ -954,35 +1010,47 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
         const uint32_t r = found;
         if (r == 0xFFFFFFFFu || h >= a.nq) continue;
         const uint32_t kvh = h / p.G;
-        // where this row's parts of an entry lie: `n` of them, a tile apart
-        auto parts = [&](const PaLeft& e, uint32_t& n) -> size_t {
+        // This row's parts of an entry: `n` places for them, not all in use.  Few rows: the shares that its unit's blocks lie in; many
+        // rows: two shares at most to a segment, whose blocks begin within one share's length.
+        struct Parts {
+            uint32_t n, row, first, k0;
+        };
+        auto parts = [&](const PaLeft& e) -> Parts {
             const uint32_t row = (t - e.t0) * p.G + h % p.G;
-            if (row >= e.rows) {  // (a request of no group)
-                n = 0;
-                return 0;
-            }
-            const uint32_t first = e.w0 + (kvh * e.tiles + row / e.tile) * e.unit + e.fix, k0 = first / e.per;
-            n = (first + (e.blocks - 1) * e.block) / e.per - k0 + 1;
-            return (size_t)e.row0 + kvh * e.rows + row + (size_t)k0 * e.tile;
+            if (row >= e.rows) return {0, 0, 0, 0};  // (a request of no group)
+            const uint32_t first = e.w0 + (kvh * e.segs * e.tiles + row / e.tile) * e.unit + e.fix, k0 = first / e.per;
+            return {e.few ? (first + (e.blocks - 1) * e.block) / e.per - k0 + 1 : 2 * e.segs, row, first, k0};
+        };
+        auto place = [&](const PaLeft& e, const Parts& x, uint32_t i, bool& used) -> size_t {
+            if (e.few) return used = true, (size_t)e.row0 + kvh * e.rows + x.row + (size_t)(x.k0 + i) * e.tile;
+            const uint32_t seg = i / 2, first = x.first + seg * e.tiles * e.unit, k = first / e.per + i % 2;
+            used = i % 2 == 0 || (first + (min(e.seg, e.blocks - seg * e.seg) - 1) * e.block) / e.per == k;
+            return (size_t)e.row0 + (size_t)(kvh * e.segs + seg) * e.rows + x.row + (size_t)k * e.tile;
         };
         const PaLeft rest = p.entries[a.n_groups + r];
-        uint32_t n0 = 0, n1, tile0 = 0;
-        size_t p0 = 0;
+        PaLeft shared;
+        Parts x0 = {0, 0, 0, 0};
         if (rest.parts) {
-            const PaLeft shared = p.entries[pa_group_of(a, r)];
-            p0 = parts(shared, n0);
-            tile0 = shared.tile;
+            shared = p.entries[pa_group_of(a, r)];
+            x0 = parts(shared);
         }
-        const size_t p1 = parts(rest, n1);
-        if (!rest.parts && n1 <= 1) continue;  // (written by the one that had it)
-        const uint32_t n = n0 + n1;
+        const Parts x1 = parts(rest);
+        if (!rest.parts) {  // written by the one that had it?
+            bool used = false;
+            if (rest.few ? x1.n <= 1 : rest.segs == 1 && (place(rest, x1, 1, used), !used)) continue;
+        }
+        const uint32_t n = x0.n + x1.n;
         if (n == 0) continue;
-        auto part = [&](uint32_t i) -> size_t { return i < n0 ? p0 + (size_t)i * tile0 : p1 + (size_t)(i - n0) * rest.tile; };
+        auto part = [&](uint32_t i, bool& used) -> size_t { return i < x0.n ? place(shared, x0, i, used) : place(rest, x1, i - x0.n, used); };
         float m = -INFINITY;
         for (uint32_t i0 = 0; i0 < n; i0 += 8) {
             float2 v[8];
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) v[u] = i0 + u < n ? p.ml[part(i0 + u)] : make_float2(-INFINITY, 0.f);
+            for (uint32_t u = 0; u < 8; u++) {
+                bool used = false;
+                const size_t at = i0 + u < n ? part(i0 + u, used) : 0;
+                v[u] = used ? p.ml[at] : make_float2(-INFINITY, 0.f);
+            }
 #pragma unroll
             for (uint32_t u = 0; u < 8; u++) m = v[u].x > m ? v[u].x : m;
         }
@@ -993,8 +1061,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
             float4 x[8];
 #pragma unroll
             for (uint32_t u = 0; u < 8; u++) {
-                v[u] = i0 + u < n ? p.ml[part(i0 + u)] : make_float2(-INFINITY, 0.f);
-                x[u] = i0 + u < n ? *reinterpret_cast<const float4*>(p.o + part(i0 + u) * HD + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                bool used = false;
+                const size_t at = i0 + u < n ? part(i0 + u, used) : 0;
+                v[u] = used ? p.ml[at] : make_float2(-INFINITY, 0.f);
+                x[u] = used ? *reinterpret_cast<const float4*>(p.o + at * HD + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
             }
 #pragma unroll
             for (uint32_t u = 0; u < 8; u++) {
@@ -1012,9 +1082,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
 }
 
 // Rows of parts at most.  The part of unit u in share k begins u's rows and k tiles behind the first one of its kind: no two overlap,
-// because the next part is of the next unit or in the next share, and no unit has more rows than a tile.
+// because the next part is of the next unit or in the next share, and no unit has more rows than a tile.  Segments beyond an entry's first
+// stand for a share's work each, of which there are PA_SHARES.
 static uint64_t most_rows(const oxb_paged_attention& a) {
-    return (uint64_t)a.n_tokens * a.nq * (a.n_groups ? 2 : 1) + (uint64_t)PA_SHARES * (pa_tile_many(a.pool.hd) + 4 * PA_TILE_FEW);
+    return (uint64_t)a.n_tokens * a.nq * (a.n_groups ? 2 : 1) + (uint64_t)PA_SHARES * (2 * pa_tile_many(a.pool.hd) + 4 * PA_TILE_FEW);
 }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static size_t entries_bytes(const oxb_paged_attention& a) { return up256(((size_t)a.n_groups + a.n_requests) * sizeof(PaLeft)); }
@@ -1049,8 +1120,8 @@ hipError_t oxb_launch_paged_attention(const oxb_paged_attention& a, hipStream_t 
     p.negative = a.scale < 0.f ? 0x80000000u : 0u;
     p.page_shift = (uint32_t)__builtin_ctz(a.pool.page_size);
     p.tile_many = pa_tile_many(a.pool.hd);
-    p.keys_many = pa_keys_many(a.pool.hd);
-    p.cost = a.pool.kv_dtype == OXB_KV_F16 ? PaCosts{1, 2, 2, 4} : PaCosts{1, 4, 2, 8};
+    p.keys_many = pa_keys_many(a.pool.hd, a.pool.kv_dtype != OXB_KV_F16, a.dtype == OXB_DTYPE_F32);
+    p.cost = {1, a.pool.kv_dtype == OXB_KV_F16 && p.keys_many == 64 ? 2u : 2u, 2, 4};
     uint8_t* ws = reinterpret_cast<uint8_t*>(a.d_workspace);
     p.entries = reinterpret_cast<PaLeft*>(ws);
     ws += entries_bytes(a);
