@@ -56,12 +56,12 @@ int check_attention_counts(const oxb_paged_attention& a) {
     if (a.n_groups > a.n_requests) return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: %u groups of %u requests", a.n_groups, a.n_requests);
     if (a.nq == 0 || a.nq % a.pool.nkv || a.nq / a.pool.nkv > OXB_PAGED_MAX_GROUP)
         return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: %u q heads over %u kv heads (1 .. %u to each)", a.nq, a.pool.nkv, OXB_PAGED_MAX_GROUP);
-    if (a.n_tokens == 0 || (uint64_t)a.n_tokens * a.nq > (1u << 30))
+    if (a.n_tokens == 0 || (uint64_t)a.n_tokens * a.nq > (1u << 30))  // (rows of parts are counted in 32 bits)
         return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: %u queries of %u heads (1 .. 2^30 rows)", a.n_tokens, a.nq);
     if (a.dtype > OXB_DTYPE_BF16) return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: type %u", a.dtype);
     if (a.table_width == 0 || (uint64_t)a.table_width * a.pool.page_size > 0x7FFFFFFFu) return bad("table rows of no entries, or of 2^31 positions and more");
     // the kernel counts the call's work in 32 bits: about a unit for 16 rows and 32 keys
-    const double tiles = (double)a.n_tokens * (a.nq / a.pool.nkv) / 16 + a.n_requests + a.n_groups, blocks = (double)a.table_width * a.pool.page_size / 32 + 10;
+    const double tiles = (double)a.n_tokens * (a.nq / a.pool.nkv) / 16 + a.n_requests + a.n_groups, blocks = (double)a.table_width * a.pool.page_size / 32 + 20;
     if ((a.n_groups ? 2 : 1) * tiles * a.pool.nkv * blocks >= 2147483648.0) return bad("more work than one call takes: too many queries over tables too wide");
     return OXB_HIP_OK;
 }

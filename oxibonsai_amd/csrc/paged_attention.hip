@@ -35,6 +35,8 @@ typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 #define PA_TILE_FEW 16u
 #define PA_KEYS_FEW 32u    // keys that such a wave takes at a time
 #define PA_RUNS 256u       // runs of entries, one to a thread
+#define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk
+#define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes
 #define PA_LOG2E 1.44269504088896340736f
 
 // Tiles of many rows and the keys of a block of theirs: what the registers and two workgroups' LDS hold.
@@ -62,8 +64,9 @@ struct PaParams {
 
 struct PaEntry {
     uint32_t t0, tn;    // queries
-    uint32_t k0, k1;    // keys
-    uint32_t table;     // row of the page tables
+    uint32_t ps;        // keys 0 .. ps - 1 through the table row of the group's first request
+    uint32_t k0, k1;    // and keys k0 .. k1 - 1 (k0 >= ps) through the own one
+    uint32_t table0, table;
     bool parts;         // the rows have another part elsewhere
     bool bad;           // sums that do not ascend
 };
@@ -71,7 +74,7 @@ struct PaEntry {
 // How an entry is cut.
 struct PaCut {
     uint32_t rows, tile, tiles;     // rows of a kv head, of a tile; tiles
-    uint32_t keys, b0, blocks;      // keys of a block; the first block; how many
+    uint32_t keys, shared, blocks;  // keys of a block; blocks of the group's keys, of all
     uint32_t segs, seg;             // segments; blocks of one, the last one may have fewer
     uint32_t block, fix, unit;      // work of a block, of a unit without its blocks, of a unit
     uint32_t units;
@@ -88,11 +91,21 @@ struct PaLeft {
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 __device__ __forceinline__ uint32_t pa_clamp(int v, uint32_t hi) { return v < 0 ? 0u : min((uint32_t)v, hi); }
 
-// Group g's requests and keys: shared by two requests or more, else the prefix is part of the rest.
-__device__ __forceinline__ uint32_t pa_shared(const oxb_paged_attention& a, uint32_t g, uint32_t& r0, uint32_t& r1) {
-    r0 = pa_clamp(a.d_cu_groups[g], a.n_requests);
-    r1 = pa_clamp(a.d_cu_groups[g + 1], a.n_requests);
-    return r1 >= r0 + 2 ? pa_clamp(a.d_prefix_lens[g], a.table_width * a.pool.page_size) : 0u;
+// Group g's requests, and the length of its prefix.  The prefix is an entry of its own if two requests or more share it and they have
+// few rows each; those of many rows fill tiles of their own and walk it themselves, in one go with their rests: no parts to add.
+struct PaGroup {
+    uint32_t r0, r1, prefix;
+    bool together;
+};
+__device__ __forceinline__ PaGroup pa_group(const PaParams& p, uint32_t g) {
+    const oxb_paged_attention& a = p.a;
+    PaGroup x;
+    x.r0 = pa_clamp(a.d_cu_groups[g], a.n_requests);
+    x.r1 = pa_clamp(a.d_cu_groups[g + 1], a.n_requests);
+    x.prefix = x.r1 > x.r0 ? pa_clamp(a.d_prefix_lens[g], a.table_width * a.pool.page_size) : 0u;
+    const uint32_t t0 = pa_clamp(a.d_cu_tokens[x.r0], a.n_tokens), t1 = pa_clamp(a.d_cu_tokens[x.r1], a.n_tokens);
+    x.together = x.prefix > 0 && x.r1 >= x.r0 + 2 && t1 > t0 && (uint64_t)(t1 - t0) * p.G < (uint64_t)(x.r1 - x.r0) * PA_OWN;
+    return x;
 }
 __device__ __forceinline__ uint32_t pa_group_of(const oxb_paged_attention& a, uint32_t r) {
     uint32_t lo = 0, hi = a.n_groups - 1;
@@ -103,28 +116,36 @@ __device__ __forceinline__ uint32_t pa_group_of(const oxb_paged_attention& a, ui
     }
     return lo;
 }
-// Entry e: the groups' prefixes first, then the requests' rests.
-__device__ __forceinline__ PaEntry pa_entry(const oxb_paged_attention& a, uint32_t e) {
+// Entry e: the groups' prefixes first, then the requests.
+__device__ __forceinline__ PaEntry pa_entry(const PaParams& p, uint32_t e) {
+    const oxb_paged_attention& a = p.a;
     PaEntry x;
     uint32_t r0, r1;
-    x.bad = false;
     if (e < a.n_groups) {
+        const PaGroup g = pa_group(p, e);
         x.bad = a.d_cu_groups[e + 1] < a.d_cu_groups[e];
-        x.k0 = 0;
-        x.k1 = pa_shared(a, e, r0, r1);
+        r0 = g.r0;
+        r1 = g.together ? g.r1 : r0;
+        x.ps = x.k0 = x.k1 = g.prefix;
+        x.table0 = x.table = r0;
         x.parts = true;
-        x.table = r0;
-        if (x.k1 == 0) r1 = r0;
     } else {
         r0 = e - a.n_groups;
         r1 = r0 + 1;
-        uint32_t g0 = 0, g1 = 0;
-        x.k0 = a.n_groups ? pa_shared(a, pa_group_of(a, r0), g0, g1) : 0u;
-        if (r0 < g0 || r0 >= g1) x.k0 = 0;  // (a request of no group)
+        x.table0 = x.table = r0;
+        x.ps = x.k0 = 0;
+        x.parts = false;
+        if (a.n_groups) {
+            const PaGroup g = pa_group(p, pa_group_of(a, r0));
+            if (r0 >= g.r0 && r0 < g.r1) {  // (else a request of no group)
+                x.parts = g.together;
+                x.k0 = g.prefix;
+                x.ps = g.together ? 0u : g.prefix;
+                x.table0 = g.r0;
+            }
+        }
         x.bad = a.d_cu_tokens[r1] < a.d_cu_tokens[r0];
         x.k1 = pa_clamp(a.d_lens[r0], a.table_width * a.pool.page_size);
-        x.parts = x.k0 > 0;
-        x.table = r0;
     }
     x.t0 = pa_clamp(a.d_cu_tokens[r0], a.n_tokens);
     const uint32_t t1 = pa_clamp(a.d_cu_tokens[r1], a.n_tokens);
@@ -141,8 +162,9 @@ __device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x, uin
     c.block = c.few ? p.cost.few : p.cost.many;
     c.fix = c.few ? p.cost.few_unit : p.cost.many_unit;
     c.tiles = (c.rows + c.tile - 1) / c.tile;
-    c.b0 = x.k0 / c.keys;
-    c.blocks = x.k1 > x.k0 ? (x.k1 + c.keys - 1) / c.keys - c.b0 : 1u;  // (a rest without keys is one block, in which nothing is seen)
+    c.shared = (x.ps + c.keys - 1) / c.keys;
+    c.blocks = c.shared + (x.k1 > x.k0 ? (x.k1 + c.keys - 1) / c.keys - x.k0 / c.keys : 0u);
+    c.blocks = c.blocks ? c.blocks : 1u;  // (rows without keys: one block, in which nothing is seen)
     c.segs = c.few ? 1u : (c.blocks * c.block + length - 1) / length;
     c.seg = (c.blocks + c.segs - 1) / c.segs;
     c.segs = (c.blocks + c.seg - 1) / c.seg;
@@ -173,7 +195,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     bool bad = false;
     PaEntry first;
     for (uint32_t e = e0; e < e1; e++) {
-        const PaEntry x = pa_entry(a, e);
+        const PaEntry x = pa_entry(p, e);
         const PaCut c = pa_cut(p, x, 0xFFFFFFFFu);
         if (e == e0) lds.first[tid] = first = x;
         bad |= x.bad;
@@ -186,7 +208,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     pl.length = uniform(max((lds.sum[0] + lds.sum[1] + lds.sum[2] + lds.sum[3] + PA_SHARES - 1) / PA_SHARES, p.cost.many));
     uint32_t work[2] = {0, 0}, rows[2] = {0, 0};
     for (uint32_t e = e0; e < e1; e++) {
-        const PaCut c = pa_cut(p, e == e0 ? first : pa_entry(a, e), pl.length);
+        const PaCut c = pa_cut(p, e == e0 ? first : pa_entry(p, e), pl.length);
         work[c.few] += c.unit * c.units;
         rows[c.few] += c.rows * c.segs * a.pool.nkv;
     }
@@ -229,7 +251,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     if (bad) pl.work = 0;
     if (leave_entries) {
         for (uint32_t e = e0; e < e1; e++) {
-            const PaEntry x = pa_entry(a, e);
+            const PaEntry x = pa_entry(p, e);
             const PaCut c = pa_cut(p, x, pl.length);
             const int f = c.few;
             p.entries[e] = {w0[f], row0[f], bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.segs, c.seg, c.block, c.fix, c.unit, x.t0, x.parts, f ? pl.share / 4 : pl.share, c.few, 0};
@@ -266,10 +288,11 @@ __device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, con
         if (w - r.w0 < n || ++e >= E) break;
         r.w0 += n;
         r.row0 += n ? r.c.rows * r.c.segs * a.pool.nkv : 0u;
-        r.x = pa_entry(a, e);
+        r.x = pa_entry(p, e);
     }
     // the same for the whole wave: into scalar registers
     r.x.t0 = uniform(r.x.t0), r.x.tn = uniform(r.x.tn), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1), r.x.table = uniform(r.x.table);
+    r.x.ps = uniform(r.x.ps), r.x.table0 = uniform(r.x.table0);
     r.x.parts = uniform(r.x.parts) != 0;
     r.c = pa_cut(p, r.x, pl.length);
     r.w0 = uniform(r.w0), r.row0 = uniform(r.row0);
@@ -280,10 +303,23 @@ __device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, con
 struct PaItem {
     PaEntry x;
     uint32_t rows, row0, kvh;  // rows of a kv head; the tile's first
-    uint32_t b0, b1;
+    uint32_t b0, b1, shared;   // (of the entry's blocks, the first `shared` of which are the group's keys)
     size_t part;               // where the tile's rows of parts begin
     bool parts;
 };
+// Block i: keys b * keys .., of which those in lo .. hi - 1 count, through a row of the page tables.
+struct PaSpan {
+    uint32_t b, lo, hi, table;
+};
+__device__ __forceinline__ PaSpan pa_span(const PaItem& it, uint32_t keys, uint32_t i) {
+    const bool s = i < it.shared;
+    return {s ? i : it.x.k0 / keys + (i - it.shared), s ? 0u : it.x.k0, s ? it.x.ps : it.x.k1, s ? it.x.table0 : it.x.table};
+}
+// Blocks in front of which all keys below `most` lie.
+__device__ __forceinline__ uint32_t pa_until(const PaItem& it, uint32_t keys, uint32_t most) {
+    if (most <= it.x.k0 || it.x.k1 <= it.x.k0) return (min(most, it.x.ps) + keys - 1) / keys;
+    return it.shared + (min(most, it.x.k1) + keys - 1) / keys - it.x.k0 / keys;
+}
 // The items of a share [w, end) of one kind of work, one after the other; k: the share's number among those of its size.
 template <typename F>
 __device__ __forceinline__ void pa_walk(const PaParams& p, const PaPlan& pl, const PaPlanLds& lds, uint32_t few, uint32_t w, uint32_t end, uint32_t k, F item) {
@@ -302,8 +338,9 @@ __device__ __forceinline__ void pa_walk(const PaParams& p, const PaPlan& pl, con
                 it.rows = c.rows;
                 it.kvh = u / c.tiles / c.segs;
                 it.row0 = tile * c.tile;
-                it.b0 = c.b0 + seg * c.seg + i0;
-                it.b1 = c.b0 + seg * c.seg + i1;
+                it.b0 = seg * c.seg + i0;
+                it.b1 = seg * c.seg + i1;
+                it.shared = c.shared;
                 it.parts = at.x.parts || c.segs > 1 || i0 != 0 || i1 != n;
                 it.part = (size_t)at.row0 + (size_t)(u / c.tiles) * c.rows + it.row0 + (size_t)k * c.tile;
                 item(it);
@@ -313,23 +350,28 @@ __device__ __forceinline__ void pa_walk(const PaParams& p, const PaPlan& pl, con
     }
 }
 
-// Eight values of q from memory, as fp32, times the scale's sign.
-__device__ __forceinline__ void pa_load_q8(const void* q, uint32_t dtype, uint32_t sign, size_t at, float v[8]) {
-    if (dtype == OXB_DTYPE_F32) {
-        const float4* s = reinterpret_cast<const float4*>(reinterpret_cast<const float*>(q) + at);
-        const float4 x = s[0], y = s[1];
-        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-    } else {
-        const v4w w = *reinterpret_cast<const v4w*>(reinterpret_cast<const uint16_t*>(q) + at);
+// Eight values of q: on their way from memory (F32: as fp32 numbers, else 16 bits each), then as fp32 times the scale's sign.
+template <bool F32>
+struct PaQ8 {
+    v4w w[F32 ? 2 : 1];
+    __device__ __forceinline__ void request(const void* q, size_t at) {
+        const v4w* s = reinterpret_cast<const v4w*>(reinterpret_cast<const uint8_t*>(q) + at * (F32 ? 4 : 2));
+#pragma unroll
+        for (int i = 0; i < (F32 ? 2 : 1); i++) w[i] = s[i];
+    }
+    __device__ __forceinline__ void values(uint32_t dtype, uint32_t sign, float v[8]) const {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const uint32_t b = i & 1 ? w[i / 2] >> 16 : w[i / 2] & 0xFFFFu;
-            v[i] = dtype == OXB_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : __uint_as_float(b << 16);
+            if constexpr (F32) {
+                v[i] = __uint_as_float(w[i / 4][i % 4] ^ sign);
+            } else {
+                const uint32_t b = i & 1 ? w[0][i / 2] >> 16 : w[0][i / 2] & 0xFFFFu;
+                v[i] = dtype == OXB_DTYPE_F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)b) : __uint_as_float(b << 16);
+                v[i] = __uint_as_float(__float_as_uint(v[i]) ^ sign);
+            }
         }
     }
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = __uint_as_float(__float_as_uint(v[i]) ^ sign);
-}
+};
 __device__ __forceinline__ uint32_t pa_bits16(float v, uint32_t dtype) {
     if (dtype == OXB_DTYPE_F16) return __builtin_bit_cast(uint16_t, (_Float16)v);
     const uint32_t u = __float_as_uint(v);
@@ -396,25 +438,32 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
     constexpr uint32_t ROWB = HD * (QC ? 1 : 2);
     const oxb_paged_attention& a = p.a;
     const uint32_t lane = threadIdx.x & 63u, c = lane & 15u, g = lane >> 4;
-    const uint32_t lo = it.x.k0, kvh = it.kvh;
+    const uint32_t kvh = it.kvh;
 
-    const int32_t* const table_row = a.d_tables + (size_t)it.x.table * a.table_width;
+    // this lane's row: requested first, looked at while the first keys travel
+    const uint32_t row = it.row0 + c;
+    const bool there = row < it.rows;
+    const uint32_t tok = it.x.t0 + (there ? row : it.rows - 1) / p.G, head = kvh * p.G + (there ? row : it.rows - 1) % p.G;
+    const int pos = a.d_positions[tok];
+    // q: element e of step s is dimension dim(s) + e
+    auto dim = [&](int s) -> uint32_t { return QC && KS > 1 ? 64u * (s / 2) + 16u * g + 8u * (s % 2) : 32u * s + 8u * g; };
+    PaQ8<TERMS == 2> qraw[KS];
+#pragma unroll
+    for (int s = 0; s < KS; s++) qraw[s].request(a.d_q, (size_t)tok * a.q_stride + (size_t)head * HD + dim(s));
+
     typedef const __attribute__((address_space(4))) int32_t* ConstInts;  // (nothing writes the tables meanwhile: scalar loads)
-    const ConstInts table = (ConstInts)(uintptr_t)table_row;
+    const ConstInts tables = (ConstInts)(uintptr_t)a.d_tables;
     const uint8_t* const Kc = reinterpret_cast<const uint8_t*>(a.pool.d_k);
     const uint8_t* const Vc = reinterpret_cast<const uint8_t*>(a.pool.d_v);
-    const uint32_t last = it.x.k1 - 1;  // (only used where there are keys)
-    // First row of the 16 positions from `at` on, which lie in one page.
-    auto row_of = [&](uint32_t at) -> size_t {
-        const uint32_t page = (uint32_t)table[at >> p.page_shift], safe = min(page, a.pool.n_pages - 1);
-        return (((size_t)kvh * a.pool.n_pages + safe) << p.page_shift) + (at & (a.pool.page_size - 1u));
-    };
-    auto request = [&](Block& B, uint32_t b) {
+    auto request = [&](Block& B, uint32_t i) {
+        const PaSpan sp = pa_span(it, 32u, i);
+        const uint32_t last = sp.hi - 1;
 #pragma unroll
         for (uint32_t kt = 0; kt < 2; kt++) {
-            // rows in front of the entry's first key or behind its last one are not read: they need hold no numbers
-            const uint32_t at = max(min(b * 32u + 16 * kt, last & ~15u), lo & ~15u), to = min(last - at, 15u), from = min(lo > at ? lo - at : 0u, to);
-            const size_t r = row_of(at);
+            // rows in front of the first key or behind the last one are not read: they need hold no numbers.  16 positions lie in one page.
+            const uint32_t at = max(min(sp.b * 32u + 16 * kt, last & ~15u), sp.lo & ~15u), to = min(last - at, 15u), from = min(sp.lo > at ? sp.lo - at : 0u, to);
+            const uint32_t page = (uint32_t)tables[(size_t)sp.table * a.table_width + (at >> p.page_shift)], safe = min(page, a.pool.n_pages - 1);
+            const size_t r = (((size_t)kvh * a.pool.n_pages + safe) << p.page_shift) + (at & (a.pool.page_size - 1u));
             const uint8_t *kr = Kc + r * ROWB, *vr = Vc + r * ROWB;
             const uint32_t kc = max(min(c, to), from) * ROWB;
 #pragma unroll
@@ -433,24 +482,17 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
     };
     // (two blocks of wide rows do not fit the registers)
     constexpr bool AHEAD = HD < 256;
-    const bool any = it.x.k1 > lo;
+    const bool any = it.x.ps > 0 || it.x.k1 > it.x.k0;
     Block A, B;
     if (any) request(A, it.b0);
 
-    // this lane's row
-    const uint32_t row = it.row0 + c;
-    const bool there = row < it.rows;
-    const uint32_t tok = it.x.t0 + (there ? row : it.rows - 1) / p.G, head = it.kvh * p.G + (there ? row : it.rows - 1) % p.G;
-    const int pos = a.d_positions[tok];
-    // q: element e of step s is dimension dim(s) + e
-    auto dim = [&](int s) -> uint32_t { return QC && KS > 1 ? 64u * (s / 2) + 16u * g + 8u * (s % 2) : 32u * s + 8u * g; };
     v8h q[TERMS][KS];
     float mul;
     {
         float f[KS][8], top = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            pa_load_q8(a.d_q, a.dtype, p.negative, (size_t)tok * a.q_stride + (size_t)head * HD + dim(s), f[s]);
+            qraw[s].values(a.dtype, p.negative, f[s]);
 #pragma unroll
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[s][e]));
         }
@@ -468,7 +510,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
             }
     }
 
-    const uint32_t sees = min(pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), it.x.k1);  // keys in front of this one
+    const uint32_t sees = pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u);  // keys in front of this one
     uint32_t most = there ? sees : 0u, least = there ? sees : 0xFFFFFFFFu;
 #pragma unroll
     for (int d = 1; d < 16; d *= 2) {
@@ -477,12 +519,13 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
     }
     most = uniform(most);
     least = uniform(least);
-    const uint32_t b1 = any ? min(it.b1, (most + 31u) / 32u) : 0u;  // (nothing is seen behind)
+    const uint32_t b1 = any ? min(it.b1, pa_until(it, 32u, most)) : 0u;  // (nothing is seen behind)
     v4f O[DPL];
 #pragma unroll
     for (int j = 0; j < DPL; j++) O[j] = (v4f){0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
-    auto block = [&](const Block& B, uint32_t b) {
+    auto block = [&](const Block& B, uint32_t i) {
+        const PaSpan sp = pa_span(it, 32u, i);
         v4f S[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
         for (int s = 0; s < KS; s++)
@@ -499,8 +542,8 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
                 for (int t = 0; t < TERMS; t++) S[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(K, q[t][s], S[kt], 0, 0, 0);
             }
         float vs[2][4], top = -INFINITY;
-        const uint32_t key0 = b * 32u;
-        const bool all = key0 >= lo && key0 + 32u <= least;  // (wave-uniform) every row sees all of these keys
+        const uint32_t key0 = sp.b * 32u;
+        const bool all = key0 >= sp.lo && key0 + 32u <= min(least, sp.hi);  // (wave-uniform) every row sees all of these keys
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
@@ -509,7 +552,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
                 if constexpr (QC) s *= B.ks[kt][v], vs[kt][v] = B.vs[kt][v];
                 if (!all) {
                     const uint32_t key = key0 + 16 * kt + 4 * g + v;
-                    const bool seen = key >= lo && key < sees;
+                    const bool seen = key >= sp.lo && key < min(sees, sp.hi);
                     s = seen ? s : -INFINITY;
                     if constexpr (QC) vs[kt][v] = seen ? vs[kt][v] : 1.f;
                 }
@@ -642,44 +685,62 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
     const oxb_paged_attention& a = p.a;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, c = lane & 15u, g = lane >> 4;
     const uint32_t wave = uniform(tid >> 6);
-    const uint32_t lo = it.x.k0, kvh = it.kvh;
+    const uint32_t kvh = it.kvh;
 
-    const int32_t* const table = a.d_tables + (size_t)it.x.table * a.table_width;
+    // this lane's rows: requested first, looked at while the first keys travel
+    uint32_t tok[QT], head[QT];
+    int pos[QT];
+    bool there[QT];
+    PaQ8<TERMS == 2> qraw[QT][KS];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+        const uint32_t row = it.row0 + (t * 4 + wave) * 16 + c, r = min(row, it.rows - 1);
+        there[t] = row < it.rows;
+        tok[t] = it.x.t0 + r / p.G;
+        head[t] = kvh * p.G + r % p.G;
+        pos[t] = a.d_positions[tok[t]];
+#pragma unroll
+        for (int s = 0; s < KS; s++) qraw[t][s].request(a.d_q, (size_t)tok[t] * a.q_stride + (size_t)head[t] * HD + 32 * s + 8 * g);
+    }
+
     const uint8_t* const Kc = reinterpret_cast<const uint8_t*>(a.pool.d_k);
     const uint8_t* const Vc = reinterpret_cast<const uint8_t*>(a.pool.d_v);
     _Float16 *const ks0 = st.k0, *const vs0 = st.v0, *const ks1 = st.k1, *const vs1 = st.v1;
-    const uint32_t last = it.x.k1 - 1;  // (only used where there are keys)
-    // this wave's rows of block b: positions `at` .. in one page; those in front of the first key or behind the last one are not read
-    auto at_of = [&](uint32_t b) -> uint32_t { return max(min(b * KB + wave * RPW, last & ~(uint32_t)(RPW - 1)), lo & ~(uint32_t)(RPW - 1)); };
+    // this wave's rows of a block: positions `at` .. in one page; those in front of the first key or behind the last one are not read
+    auto at_of = [&](const PaSpan& sp) -> uint32_t { return max(min(sp.b * KB + wave * RPW, (sp.hi - 1) & ~(uint32_t)(RPW - 1)), sp.lo & ~(uint32_t)(RPW - 1)); };
     // The page of the next request travels with the rows of the one before.
-    auto page_of = [&](uint32_t b) -> uint32_t { return (uint32_t)table[at_of(b) >> p.page_shift]; };
     uint32_t page = 0;
-    auto rows_of = [&](uint32_t b, uint32_t& from, uint32_t& to) -> size_t {
-        const uint32_t at = at_of(b);
-        to = min(last - at, (uint32_t)RPW - 1);
-        from = min(lo > at ? lo - at : 0u, to);
+    auto page_of = [&](uint32_t i) {
+        if (i >= it.b1) return;
+        const PaSpan sp = pa_span(it, KB, i);
+        page = (uint32_t)a.d_tables[(size_t)sp.table * a.table_width + (at_of(sp) >> p.page_shift)];
+    };
+    auto rows_of = [&](const PaSpan& sp, uint32_t& from, uint32_t& to) -> size_t {
+        const uint32_t at = at_of(sp);
+        to = min(sp.hi - 1 - at, (uint32_t)RPW - 1);
+        from = min(sp.lo > at ? sp.lo - at : 0u, to);
         return (((size_t)kvh * a.pool.n_pages + min(uniform(page), a.pool.n_pages - 1)) << p.page_shift) + (at & (a.pool.page_size - 1u));
     };
     v4w kreg[QC ? NI : 1], vreg[QC ? NI : 1];
     float kscale = 0.f, vscale = 0.f;
-    auto request = [&](uint32_t b, _Float16* kd, _Float16* vd) {
+    auto request = [&](uint32_t i, _Float16* kd, _Float16* vd) {
         uint32_t from, to;
-        const size_t row = rows_of(b, from, to);
+        const size_t row = rows_of(pa_span(it, KB, i), from, to);
         const uint8_t *kb = Kc + row * ROWB, *vb = Vc + row * ROWB;
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
+        for (int j = 0; j < NI; j++) {
             constexpr uint32_t SPR = ROWB / 16;  // pieces of a cache row
-            const uint32_t id = i * 64 + lane, r = id / SPR, piece = QC ? id % SPR : (id % SPR) ^ (((wave * RPW + r) / RB) & PM);
+            const uint32_t id = j * 64 + lane, r = id / SPR, piece = QC ? id % SPR : (id % SPR) ^ (((wave * RPW + r) / RB) & PM);
             const uint32_t off = max(min(r, to), from) * ROWB + piece * 16;
             if (HALF && lane >= RPW * ROWB / 16) continue;
             if constexpr (QC) {
-                kreg[i] = *reinterpret_cast<const v4w*>(kb + off);
-                vreg[i] = *reinterpret_cast<const v4w*>(vb + off);
+                kreg[j] = *reinterpret_cast<const v4w*>(kb + off);
+                vreg[j] = *reinterpret_cast<const v4w*>(vb + off);
             } else {
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(kb + off),
-                                                 (__attribute__((address_space(3))) void*)(kd + (wave * RPW * PPR + i * 64) * 8), 16, 0, 0);
+                                                 (__attribute__((address_space(3))) void*)(kd + (wave * RPW * PPR + j * 64) * 8), 16, 0, 0);
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(vb + off),
-                                                 (__attribute__((address_space(3))) void*)(vd + (wave * RPW * PPR + i * 64) * 8), 16, 0, 0);
+                                                 (__attribute__((address_space(3))) void*)(vd + (wave * RPW * PPR + j * 64) * 8), 16, 0, 0);
             }
         }
         if constexpr (QC) {
@@ -687,7 +748,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             kscale = a.pool.d_k_scale[row + r];
             vscale = a.pool.d_v_scale[row + r];
         }
-        page = page_of(b + 1);
+        page_of(i + 1);
     };
     // The barrier that ends a block: every wave has read it, and the next one is complete in LDS.
     auto deliver = [&](_Float16* kd, _Float16* vd, float* sc, bool there_is) {
@@ -715,23 +776,15 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     };
 
-    const bool any = it.x.k1 > lo;
+    const bool any = it.x.ps > 0 || it.x.k1 > it.x.k0;
+    if (any) page_of(it.b0);
     __syncthreads();  // (the item before has been read)
-    if (any) {
-        page = page_of(it.b0);
-        request(it.b0, ks0, vs0);
-    }
+    if (any) request(it.b0, ks0, vs0);
 
-    uint32_t tok[QT], head[QT], sees[QT], most = 0, least = 0xFFFFFFFFu;
-    bool there[QT];
+    uint32_t sees[QT], most = 0, least = 0xFFFFFFFFu;
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-        const uint32_t row = it.row0 + (t * 4 + wave) * 16 + c, r = min(row, it.rows - 1);
-        there[t] = row < it.rows;
-        tok[t] = it.x.t0 + r / p.G;
-        head[t] = kvh * p.G + r % p.G;
-        const int pos = a.d_positions[tok[t]];
-        sees[t] = min(pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), it.x.k1);
+        sees[t] = pa_clamp(pos[t], 0x7FFFFFFEu) + (pos[t] >= 0 ? 1u : 0u);
         most = max(most, there[t] ? sees[t] : 0u);
         least = min(least, there[t] ? sees[t] : 0xFFFFFFFFu);
     }
@@ -751,7 +804,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
         float f[KS][8], top = 0.f;
 #pragma unroll
         for (int s = 0; s < KS; s++) {
-            pa_load_q8(a.d_q, a.dtype, p.negative, (size_t)tok[t] * a.q_stride + (size_t)head[t] * HD + 32 * s + 8 * g, f[s]);
+            qraw[t][s].values(a.dtype, p.negative, f[s]);
 #pragma unroll
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[s][e]));
         }
@@ -782,8 +835,9 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
         m[t] = -INFINITY;
         l[t] = 0.f;
     }
-    auto block = [&](const _Float16* kb, const _Float16* vb, const float* sc, uint32_t b) {
-        const uint32_t key0 = b * KB;
+    auto block = [&](const _Float16* kb, const _Float16* vb, const float* sc, uint32_t i) {
+        const PaSpan sp = pa_span(it, KB, i);
+        const uint32_t key0 = sp.b * KB;
         if (key0 >= most) return;  // (wave-uniform) nothing for this wave's rows
         // Operands are requested ahead of their use, and the fences hold the compiler to that order: K of the next 32 keys right after
         // its registers' last use, V in groups of VB, the first of them while the probabilities are worked out.
@@ -828,7 +882,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             }
         read_v(0);
         fence();
-        const bool all = key0 >= lo && key0 + KB <= least;  // (wave-uniform) every row sees all of these keys
+        const bool all = key0 >= sp.lo && key0 + KB <= min(least, sp.hi);  // (wave-uniform) every row sees all of these keys
         v8h P[TERMS][QT][NH];
         float vs[NT][4];
 #pragma unroll
@@ -851,7 +905,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
                 for (int v = 0; v < 4; v++) {
                     const uint32_t key = key0 + 16 * kt + 4 * g + v;
 #pragma unroll
-                    for (int t = 0; t < QT; t++) S[t][kt][v] = key >= lo && key < sees[t] ? S[t][kt][v] : -INFINITY;
+                    for (int t = 0; t < QT; t++) S[t][kt][v] = key >= sp.lo && key < min(sees[t], sp.hi) ? S[t][kt][v] : -INFINITY;
                 }
         }
         // (the tiles side by side: one's latencies are the other's work)
@@ -939,7 +993,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
         deliver(ks0, vs0, sc0, true);
         // nothing is seen behind the last query's keys
         const uint32_t wg_most = uniform(max(max(plan_lds.most[0], plan_lds.most[1]), max(plan_lds.most[2], plan_lds.most[3])));
-        const uint32_t b1 = min(it.b1, (wg_most + KB - 1) / KB);
+        const uint32_t b1 = min(it.b1, pa_until(it, KB, wg_most));
         for (uint32_t b = it.b0; b < b1;) {
             if (b + 1 < b1) request(b + 1, ks1, vs1);
             block(ks0, vs0, sc0, b);
@@ -991,16 +1045,20 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 }
 
 // ---------------------------------------------------------------------------
-// The parts of every row brought to a common maximum and added in order: the prefix' parts, then the rest's.  HD / 4 lanes to a row.
+// The parts of every row brought to a common maximum and added in order: the prefix' parts, then the rest's.  HD / 4 lanes to a row and
+// every GROUPS-th part, whose sums meet in LDS: eight where the rows are few and may have been cut into very many parts, whose reads
+// would follow each other, else one.
 // ---------------------------------------------------------------------------
-template <int HD>
+template <int HD, int GROUPS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
     const oxb_paged_attention& a = p.a;
-    constexpr uint32_t L = HD / 4, HPW = 256 / L;
+    constexpr uint32_t L = HD / 4, HPW = 256 / (L * GROUPS) ? 256 / (L * GROUPS) : 1;
     __shared__ uint32_t found;
-    const uint32_t tid = threadIdx.x, c = tid % L, per_tok = (a.nq + HPW - 1) / HPW;
+    __shared__ float2 part_ml[GROUPS][HPW];
+    __shared__ __attribute__((aligned(16))) float part_o[GROUPS][HPW][HD];
+    const uint32_t tid = threadIdx.x, c = tid % L, group = tid / L / HPW, per_tok = (a.nq + HPW - 1) / HPW;
     for (uint64_t w = blockIdx.x; w < (uint64_t)a.n_tokens * per_tok; w += gridDim.x) {
-        const uint32_t t = (uint32_t)(w / per_tok), h = (uint32_t)(w % per_tok) * HPW + tid / L;
+        const uint32_t t = (uint32_t)(w / per_tok), hl = tid / L % HPW, h = (uint32_t)(w % per_tok) * HPW + hl;
         __syncthreads();
         if (tid == 0) found = 0xFFFFFFFFu;
         __syncthreads();
@@ -1008,8 +1066,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
             if (a.d_cu_tokens[r] <= (int)t && (int)t < a.d_cu_tokens[r + 1]) found = r;
         __syncthreads();
         const uint32_t r = found;
-        if (r == 0xFFFFFFFFu || h >= a.nq) continue;
-        const uint32_t kvh = h / p.G;
+        if (r == 0xFFFFFFFFu) continue;
+        const uint32_t kvh = min(h, a.nq - 1) / p.G;
         // This row's parts of an entry: `n` places for them, not all in use.  Few rows: the shares that its unit's blocks lie in; many
         // rows: two shares at most to a segment, whose blocks begin within one share's length.
         struct Parts {
@@ -1035,44 +1093,70 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
             x0 = parts(shared);
         }
         const Parts x1 = parts(rest);
-        if (!rest.parts) {  // written by the one that had it?
+        uint32_t n = h < a.nq ? x0.n + x1.n : 0u;
+        if (!rest.parts && n) {  // written by the one that had it?
             bool used = false;
-            if (rest.few ? x1.n <= 1 : rest.segs == 1 && (place(rest, x1, 1, used), !used)) continue;
+            if (rest.few ? n <= 1 : rest.segs == 1 && (place(rest, x1, 1, used), !used)) n = 0;
         }
-        const uint32_t n = x0.n + x1.n;
-        if (n == 0) continue;
         auto part = [&](uint32_t i, bool& used) -> size_t { return i < x0.n ? place(shared, x0, i, used) : place(rest, x1, i - x0.n, used); };
-        float m = -INFINITY;
-        for (uint32_t i0 = 0; i0 < n; i0 += 8) {
-            float2 v[8];
+        // a place to each lane: it works out where that is, and the row's lanes then read the places in use together
+        float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+        for (uint32_t i0 = group * L; i0 < n; i0 += L * GROUPS) {
+            bool used = false;
+            const uint32_t i = i0 + c, at = i < n ? (uint32_t)part(i, used) : 0u;
+            const float2 v = used ? p.ml[at] : make_float2(-INFINITY, 0.f);
+            float top = v.x;
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) {
-                bool used = false;
-                const size_t at = i0 + u < n ? part(i0 + u, used) : 0;
-                v[u] = used ? p.ml[at] : make_float2(-INFINITY, 0.f);
+            for (uint32_t d = 1; d < L; d *= 2) {
+                const float other = __shfl_xor(top, d, L);
+                top = other > top ? other : top;
             }
+            const float now = top > m ? top : m, ref = now == -INFINITY ? 0.f : now, by = __builtin_amdgcn_exp2f(m - ref), f = __builtin_amdgcn_exp2f(v.x - ref);
+            m = now;
+            float sum = v.y * f;
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) m = v[u].x > m ? v[u].x : m;
+            for (uint32_t d = 1; d < L; d *= 2) sum += __shfl_xor(sum, d, L);
+            l = fmaf(l, by, sum);
+#pragma unroll
+            for (int k = 0; k < 4; k++) o[k] *= by;
+            const unsigned long long all = __builtin_amdgcn_ballot_w64(used);
+            unsigned long long mine = L == 64 ? all : (all >> ((tid & 63u) / L * L)) & ((1ull << (L & 63)) - 1);
+            while (mine) {
+                float4 x[4];
+                float w4[4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    const int lane = mine ? __builtin_ctzll(mine) : 0;
+                    w4[k] = mine ? __shfl(f, lane, L) : 0.f;
+                    const uint32_t from = (uint32_t)__shfl((int)at, lane, L);
+                    x[k] = mine ? *reinterpret_cast<const float4*>(p.o + (size_t)from * HD + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                    mine &= mine - 1;
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+                    o[0] = fmaf(x[k].x, w4[k], o[0]), o[1] = fmaf(x[k].y, w4[k], o[1]), o[2] = fmaf(x[k].z, w4[k], o[2]), o[3] = fmaf(x[k].w, w4[k], o[3]);
+            }
         }
-        const float ref = m == -INFINITY ? 0.f : m;
-        float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-        for (uint32_t i0 = 0; i0 < n; i0 += 8) {
-            float2 v[8];
-            float4 x[8];
+        if constexpr (GROUPS > 1) {
+            if (c == 0) part_ml[group][hl] = make_float2(m, l);
+            *reinterpret_cast<float4*>(&part_o[group][hl][4 * c]) = make_float4(o[0], o[1], o[2], o[3]);
+            __syncthreads();
+            if (group == 0) {
+                m = -INFINITY;
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) {
-                bool used = false;
-                const size_t at = i0 + u < n ? part(i0 + u, used) : 0;
-                v[u] = used ? p.ml[at] : make_float2(-INFINITY, 0.f);
-                x[u] = used ? *reinterpret_cast<const float4*>(p.o + at * HD + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-            }
+                for (int i = 0; i < GROUPS; i++) m = part_ml[i][hl].x > m ? part_ml[i][hl].x : m;
+                const float ref = m == -INFINITY ? 0.f : m;
+                l = o[0] = o[1] = o[2] = o[3] = 0.f;
 #pragma unroll
-            for (uint32_t u = 0; u < 8; u++) {
-                const float f = __builtin_amdgcn_exp2f(v[u].x - ref);
-                l = fmaf(v[u].y, f, l);
-                o[0] = fmaf(x[u].x, f, o[0]), o[1] = fmaf(x[u].y, f, o[1]), o[2] = fmaf(x[u].z, f, o[2]), o[3] = fmaf(x[u].w, f, o[3]);
+                for (int i = 0; i < GROUPS; i++) {
+                    const float f = __builtin_amdgcn_exp2f(part_ml[i][hl].x - ref);
+                    const float4 x = *reinterpret_cast<const float4*>(&part_o[i][hl][4 * c]);
+                    l = fmaf(part_ml[i][hl].y, f, l);
+                    o[0] = fmaf(x.x, f, o[0]), o[1] = fmaf(x.y, f, o[1]), o[2] = fmaf(x.z, f, o[2]), o[3] = fmaf(x.w, f, o[3]);
+                }
             }
         }
+        if (n == 0 || group) continue;
         const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
         for (int i = 0; i < 4; i++) o[i] *= inv;
@@ -1107,8 +1191,13 @@ static hipError_t attention_launch_hd(const PaParams& p, hipStream_t st) {
     else attention_launch<HD, OXB_KV_FP8_E4M3>(p, PA_SHARES, st);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const uint64_t wgs = (uint64_t)a.n_tokens * ((a.nq + 256 / (HD / 4) - 1) / (256 / (HD / 4)));
-    hipLaunchKernelGGL(paged_merge_kernel<HD>, dim3((uint32_t)(wgs < 2048 ? wgs : 2048)), dim3(256), 0, st, p);
+    constexpr uint32_t GROUPS = HD == 256 ? 4 : 8;
+    const bool wide = (uint64_t)a.n_tokens * a.nq <= PA_MERGE_WIDE;
+    const uint32_t heads = wide ? 256 / (HD / 4 * GROUPS) : 256 / (HD / 4);
+    const uint64_t wgs = (uint64_t)a.n_tokens * ((a.nq + heads - 1) / heads);
+    const dim3 grid((uint32_t)(wgs < 4096 ? wgs : 4096));
+    if (wide) hipLaunchKernelGGL((paged_merge_kernel<HD, GROUPS>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_merge_kernel<HD, 1>), grid, dim3(256), 0, st, p);
     return hipGetLastError();
 }
 
@@ -1121,7 +1210,7 @@ hipError_t oxb_launch_paged_attention(const oxb_paged_attention& a, hipStream_t 
     p.page_shift = (uint32_t)__builtin_ctz(a.pool.page_size);
     p.tile_many = pa_tile_many(a.pool.hd);
     p.keys_many = pa_keys_many(a.pool.hd, a.pool.kv_dtype != OXB_KV_F16, a.dtype == OXB_DTYPE_F32);
-    p.cost = {1, a.pool.kv_dtype == OXB_KV_F16 && p.keys_many == 64 ? 2u : 2u, 2, 4};
+    p.cost = {1, 4, 3, 12};
     uint8_t* ws = reinterpret_cast<uint8_t*>(a.d_workspace);
     p.entries = reinterpret_cast<PaLeft*>(ws);
     ws += entries_bytes(a);
