@@ -7,17 +7,15 @@
 // sum_parts exp(m_part - m) (l_part, o_part) is the whole.  So the prefix is read once for all queries of the group, the rows of
 // its products being all (query, q head) pairs of a kv head, and only the rests are read request by request.
 //
-// Work is cut on the device, because the lengths lie there.  An entry is a group's prefix or a request's rest, a unit one tile of
-// its rows of a kv head over a segment of its keys (all of them where the rows are few).  The units' work, laid end to end, those
-// of many rows first, is dealt out in equal shares to 512 workgroups, two to a CU: every workgroup sums up the entries'
-// work, finds where its share begins and walks from there, the end of one unit, whole ones, the beginning of another.  Units of
-// many rows are walked by a workgroup, those of few rows by single waves, to each a quarter of the share.  A row whose keys
-// lie in one unit and share is written at once, other parts go to the workspace and a second launch adds them.
-// Workgroups go to the eight XCDs in turn, shares go to them in runs; a segment is about a share long and the tiles of its
-// rows follow each other, so they walk the same keys at the same time and meet in one L2 (whole walks per tile instead:
-// 2.9 us for 64 keys of 128 rows where that takes 1.2, 256 requests behind 16000 keys, every tile's keys from memory).
-// The first workgroup of a CU takes from the first half, where the prefixes are, which are bound by the matrix cores, the second
-// one from the second half, where the rests are, which are bound by memory.
+// Work is cut on the device, because the lengths lie there.  An entry is a group's prefix or a request's rest, a unit one kv head and
+// tile of rows of an entry over all its keys.  The units' work, laid end to end, those of many rows first, is dealt out in
+// equal shares to 512 workgroups, two to a CU: every workgroup sums up the entries' work, finds where its share begins and walks
+// from there, the end of one unit, whole ones, the beginning of another.  Units of many rows are walked by a workgroup,
+// those of few rows by single waves, to each a quarter of the share.  A row whose keys lie in one unit and share is written at
+// once, other parts go to the workspace and a second launch adds them.
+// Workgroups go to the eight XCDs in turn, shares go to them in runs, so that the tiles of a kv head, which walk the same keys, are near
+// each other.  The first workgroup of a CU takes from the first half, where the prefixes are, which are bound by the matrix
+// cores, the second one from the second half, where the rests are, which are bound by memory.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -32,9 +30,10 @@ typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 
 #define PA_SHARES 512u     // workgroups: two to a CU
 #define PA_FEW 32u         // rows up to which an entry's tiles have 16 rows and a wave to themselves
-#define PA_TILE_FEW 16u
-#define PA_KEYS_FEW 32u    // keys that such a wave takes at a time
+#define PA_TILE_FEW_LOG 4u
+#define PA_KEYS_FEW_LOG 5u // keys that such a wave takes at a time: 32
 #define PA_RUNS 256u       // runs of entries, one to a thread
+#define PA_STAGED 512u     // requests up to which a workgroup copies the lengths to LDS first
 #define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk
 #define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes
 #define PA_LOG2E 1.44269504088896340736f
@@ -55,7 +54,7 @@ struct PaParams {
     uint32_t negative; // the scale's sign bit, for q
     uint32_t G;        // q heads to a kv head
     uint32_t page_shift;
-    uint32_t tile_many, keys_many;
+    uint32_t tile_many_log, keys_many_log;
     PaCosts cost;
     struct PaLeft* entries;  // workspace: what the merge needs of every entry
     float2* ml;        // maximum (log2 units) and sum of every part's rows
@@ -73,9 +72,8 @@ struct PaEntry {
 
 // How an entry is cut.
 struct PaCut {
-    uint32_t rows, tile, tiles;     // rows of a kv head, of a tile; tiles
-    uint32_t keys, shared, blocks;  // keys of a block; blocks of the group's keys, of all
-    uint32_t segs, seg;             // segments; blocks of one, the last one may have fewer
+    uint32_t rows, tile, tiles;     // rows of a kv head, of a tile (as a power of two); tiles
+    uint32_t keys, shared, blocks;  // keys of a block (as a power of two); blocks of the group's keys, of all
     uint32_t block, fix, unit;      // work of a block, of a unit without its blocks, of a unit
     uint32_t units;
     bool few;
@@ -85,7 +83,7 @@ struct PaCut {
 struct PaLeft {
     uint32_t w0;                    // where the entry's work begins
     uint32_t row0;                  // ... and its rows of parts
-    uint32_t rows, tile, tiles, blocks, segs, seg, block, fix, unit, t0, parts, per, few, pad;  // per: work of a share of such units
+    uint32_t rows, tile, tiles, blocks, block, fix, unit, t0, parts, per;  // per: work of a share of such units
 };
 
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
@@ -97,33 +95,38 @@ struct PaGroup {
     uint32_t r0, r1, prefix;
     bool together;
 };
-__device__ __forceinline__ PaGroup pa_group(const PaParams& p, uint32_t g) {
+// The call's lengths, in memory or as a workgroup's copies.
+struct PaView {
+    const int32_t *cu_tokens, *lens, *cu_groups, *prefix_lens;
+};
+__device__ __forceinline__ PaGroup pa_group(const PaParams& p, const PaView& v, uint32_t g) {
     const oxb_paged_attention& a = p.a;
     PaGroup x;
-    x.r0 = pa_clamp(a.d_cu_groups[g], a.n_requests);
-    x.r1 = pa_clamp(a.d_cu_groups[g + 1], a.n_requests);
-    x.prefix = x.r1 > x.r0 ? pa_clamp(a.d_prefix_lens[g], a.table_width * a.pool.page_size) : 0u;
-    const uint32_t t0 = pa_clamp(a.d_cu_tokens[x.r0], a.n_tokens), t1 = pa_clamp(a.d_cu_tokens[x.r1], a.n_tokens);
+    x.r0 = pa_clamp(v.cu_groups[g], a.n_requests);
+    x.r1 = pa_clamp(v.cu_groups[g + 1], a.n_requests);
+    x.prefix = x.r1 > x.r0 ? pa_clamp(v.prefix_lens[g], a.table_width * a.pool.page_size) : 0u;
+    const uint32_t t0 = pa_clamp(v.cu_tokens[x.r0], a.n_tokens), t1 = pa_clamp(v.cu_tokens[x.r1], a.n_tokens);
     x.together = x.prefix > 0 && x.r1 >= x.r0 + 2 && t1 > t0 && (uint64_t)(t1 - t0) * p.G < (uint64_t)(x.r1 - x.r0) * PA_OWN;
     return x;
 }
-__device__ __forceinline__ uint32_t pa_group_of(const oxb_paged_attention& a, uint32_t r) {
+// The group of request r.
+__device__ __forceinline__ uint32_t pa_group_of(const oxb_paged_attention& a, const int32_t* cu_groups, uint32_t r) {
     uint32_t lo = 0, hi = a.n_groups - 1;
     while (lo < hi) {
         const uint32_t mid = (lo + hi) / 2;
-        if (a.d_cu_groups[mid + 1] > (int)r) hi = mid;
+        if (cu_groups[mid + 1] > (int)r) hi = mid;
         else lo = mid + 1;
     }
     return lo;
 }
 // Entry e: the groups' prefixes first, then the requests.
-__device__ __forceinline__ PaEntry pa_entry(const PaParams& p, uint32_t e) {
+__device__ __forceinline__ PaEntry pa_entry(const PaParams& p, const PaView& v, uint32_t e) {
     const oxb_paged_attention& a = p.a;
     PaEntry x;
     uint32_t r0, r1;
     if (e < a.n_groups) {
-        const PaGroup g = pa_group(p, e);
-        x.bad = a.d_cu_groups[e + 1] < a.d_cu_groups[e];
+        const PaGroup g = pa_group(p, v, e);
+        x.bad = v.cu_groups[e + 1] < v.cu_groups[e];
         r0 = g.r0;
         r1 = g.together ? g.r1 : r0;
         x.ps = x.k0 = x.k1 = g.prefix;
@@ -136,7 +139,7 @@ __device__ __forceinline__ PaEntry pa_entry(const PaParams& p, uint32_t e) {
         x.ps = x.k0 = 0;
         x.parts = false;
         if (a.n_groups) {
-            const PaGroup g = pa_group(p, pa_group_of(a, r0));
+            const PaGroup g = pa_group(p, v, pa_group_of(a, v.cu_groups, r0));
             if (r0 >= g.r0 && r0 < g.r1) {  // (else a request of no group)
                 x.parts = g.together;
                 x.k0 = g.prefix;
@@ -144,44 +147,59 @@ __device__ __forceinline__ PaEntry pa_entry(const PaParams& p, uint32_t e) {
                 x.table0 = g.r0;
             }
         }
-        x.bad = a.d_cu_tokens[r1] < a.d_cu_tokens[r0];
-        x.k1 = pa_clamp(a.d_lens[r0], a.table_width * a.pool.page_size);
+        x.bad = v.cu_tokens[r1] < v.cu_tokens[r0];
+        x.k1 = pa_clamp(v.lens[r0], a.table_width * a.pool.page_size);
     }
-    x.t0 = pa_clamp(a.d_cu_tokens[r0], a.n_tokens);
-    const uint32_t t1 = pa_clamp(a.d_cu_tokens[r1], a.n_tokens);
+    x.t0 = pa_clamp(v.cu_tokens[r0], a.n_tokens);
+    const uint32_t t1 = pa_clamp(v.cu_tokens[r1], a.n_tokens);
     x.tn = t1 > x.t0 ? t1 - x.t0 : 0u;
     return x;
 }
-// `length`: work of a segment at most.
-__device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x, uint32_t length) {
+// a / b, b > 0: from the quotient of the numbers as floats, which is off by a part in 2^21
+__device__ __forceinline__ uint32_t pa_div(uint32_t a, uint32_t b) {
+    uint32_t q = (uint32_t)((float)a * __builtin_amdgcn_rcpf((float)b));
+    while ((uint64_t)q * b > a) q--;
+    while (a - q * b >= b) q++;
+    return q;
+}
+__device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x) {
     PaCut c;
     c.rows = x.tn * p.G;
     c.few = c.rows <= PA_FEW;
-    c.tile = c.few ? PA_TILE_FEW : p.tile_many;
-    c.keys = c.few ? PA_KEYS_FEW : p.keys_many;
+    c.tile = c.few ? PA_TILE_FEW_LOG : p.tile_many_log;
+    c.keys = c.few ? PA_KEYS_FEW_LOG : p.keys_many_log;
     c.block = c.few ? p.cost.few : p.cost.many;
     c.fix = c.few ? p.cost.few_unit : p.cost.many_unit;
-    c.tiles = (c.rows + c.tile - 1) / c.tile;
-    c.shared = (x.ps + c.keys - 1) / c.keys;
-    c.blocks = c.shared + (x.k1 > x.k0 ? (x.k1 + c.keys - 1) / c.keys - x.k0 / c.keys : 0u);
+    c.tiles = (c.rows + (1u << c.tile) - 1) >> c.tile;
+    const uint32_t up = (1u << c.keys) - 1;
+    c.shared = (x.ps + up) >> c.keys;
+    c.blocks = c.shared + (x.k1 > x.k0 ? ((x.k1 + up) >> c.keys) - (x.k0 >> c.keys) : 0u);
     c.blocks = c.blocks ? c.blocks : 1u;  // (rows without keys: one block, in which nothing is seen)
-    c.segs = c.few ? 1u : (c.blocks * c.block + length - 1) / length;
-    c.seg = (c.blocks + c.segs - 1) / c.segs;
-    c.segs = (c.blocks + c.seg - 1) / c.seg;
-    c.unit = c.fix + c.seg * c.block;
-    c.units = c.tiles * c.segs * p.a.pool.nkv;
+    c.unit = c.fix + c.blocks * c.block;
+    c.units = c.tiles * p.a.pool.nkv;
     return c;
+}
+
+// Inclusive sum over the 64 lanes of a wave: four steps inside rows of 16 lanes, then the rows' last lanes to the rows behind them.
+__device__ __forceinline__ uint32_t pa_scan(uint32_t v) {
+    v += dpp_u32<OXB_DPP_ROW_SHR(1)>(v);
+    v += dpp_u32<OXB_DPP_ROW_SHR(2)>(v);
+    v += dpp_u32<OXB_DPP_ROW_SHR(4)>(v);
+    v += dpp_u32<OXB_DPP_ROW_SHR(8)>(v);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return v;
 }
 
 // The plan of a call, the same in every workgroup: thread i holds run i of the entries.
 struct PaPlanLds {
-    uint32_t sum[4], work[2][4], rows[2][4], bad[4], most[4];
+    uint32_t work[2][4], rows[2][4], bad[4], most[4];
     uint32_t w0[2][PA_RUNS], row0[2][PA_RUNS];  // where the work and the rows of parts of a run begin: those of many rows, those of few
-    PaEntry first[PA_RUNS];                     // a run's first entry
+    int32_t cu_tokens[PA_STAGED + 1], lens[PA_STAGED], cu_groups[PA_STAGED + 1], prefix_lens[PA_STAGED];
 };
 struct PaPlan {
+    PaView view;
     uint32_t work, few0, share, per;   // all work, where that of few rows begins, a workgroup's share, entries to a run
-    uint32_t length;                   // work of a segment, at most
 };
 
 __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, bool leave_entries) {
@@ -189,37 +207,28 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_groups + a.n_requests;
     PaPlan pl;
     pl.per = (E + PA_RUNS - 1) / PA_RUNS;
-    const uint32_t e0 = min(tid * pl.per, E), e1 = min(e0 + pl.per, E);
-    // the work as it were if every unit had all its keys gives the length of a segment
-    uint32_t whole = 0;
-    bool bad = false;
-    PaEntry first;
-    for (uint32_t e = e0; e < e1; e++) {
-        const PaEntry x = pa_entry(p, e);
-        const PaCut c = pa_cut(p, x, 0xFFFFFFFFu);
-        if (e == e0) lds.first[tid] = first = x;
-        bad |= x.bad;
-        whole += c.unit * c.units;
-    }
-#pragma unroll
-    for (int d = 32; d; d /= 2) whole += __shfl_xor(whole, d, 64);
-    if (lane == 0) lds.sum[wave] = whole;
-    __syncthreads();
-    pl.length = uniform(max((lds.sum[0] + lds.sum[1] + lds.sum[2] + lds.sum[3] + PA_SHARES - 1) / PA_SHARES, p.cost.many));
-    uint32_t work[2] = {0, 0}, rows[2] = {0, 0};
-    for (uint32_t e = e0; e < e1; e++) {
-        const PaCut c = pa_cut(p, e == e0 ? first : pa_entry(p, e), pl.length);
-        work[c.few] += c.unit * c.units;
-        rows[c.few] += c.rows * c.segs * a.pool.nkv;
-    }
-    uint32_t iw[2] = {work[0], work[1]}, ir[2] = {rows[0], rows[1]};
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2)
-#pragma unroll
-        for (int f = 0; f < 2; f++) {
-            const uint32_t ow = __shfl_up(iw[f], d, 64), orr = __shfl_up(ir[f], d, 64);
-            if (lane >= (uint32_t)d) iw[f] += ow, ir[f] += orr;
+    pl.view = {a.d_cu_tokens, a.d_lens, a.d_cu_groups, a.d_prefix_lens};
+    if (a.n_requests <= PA_STAGED) {  // one trip to memory for all of them
+        for (uint32_t r = tid; r <= a.n_requests; r += 256) lds.cu_tokens[r] = a.d_cu_tokens[r];
+        for (uint32_t r = tid; r < a.n_requests; r += 256) lds.lens[r] = a.d_lens[r];
+        if (a.n_groups) {
+            for (uint32_t g = tid; g <= a.n_groups; g += 256) lds.cu_groups[g] = a.d_cu_groups[g];
+            for (uint32_t g = tid; g < a.n_groups; g += 256) lds.prefix_lens[g] = a.d_prefix_lens[g];
         }
+        pl.view = {lds.cu_tokens, lds.lens, lds.cu_groups, lds.prefix_lens};
+        __syncthreads();
+    }
+    const uint32_t e0 = min(tid * pl.per, E), e1 = min(e0 + pl.per, E);
+    uint32_t work[2] = {0, 0}, rows[2] = {0, 0};
+    bool bad = false;
+    for (uint32_t e = e0; e < e1; e++) {
+        const PaEntry x = pa_entry(p, pl.view, e);
+        const PaCut c = pa_cut(p, x);
+        bad |= x.bad;
+        work[c.few] += c.unit * c.units;
+        rows[c.few] += c.rows * a.pool.nkv;
+    }
+    uint32_t iw[2] = {pa_scan(work[0]), pa_scan(work[1])}, ir[2] = {pa_scan(rows[0]), pa_scan(rows[1])};
     bad = __builtin_amdgcn_ballot_w64(bad) != 0;
     if (lane == 63) {
 #pragma unroll
@@ -242,7 +251,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     pl.few0 = uniform(all[0]);
     pl.work = uniform(all[0] + all[1]);
     w0[1] += all[0];
-    row0[1] += all_rows + PA_SHARES * p.tile_many;  // (behind the parts of many rows)
+    row0[1] += all_rows + (PA_SHARES << p.tile_many_log);  // (behind the parts of many rows)
 #pragma unroll
     for (int f = 0; f < 2; f++) lds.w0[f][tid] = w0[f], lds.row0[f][tid] = row0[f];
     // four waves to a share, and no share without a block: parts are counted by the blocks that begin in a share
@@ -251,12 +260,12 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     if (bad) pl.work = 0;
     if (leave_entries) {
         for (uint32_t e = e0; e < e1; e++) {
-            const PaEntry x = pa_entry(p, e);
-            const PaCut c = pa_cut(p, x, pl.length);
+            const PaEntry x = pa_entry(p, pl.view, e);
+            const PaCut c = pa_cut(p, x);
             const int f = c.few;
-            p.entries[e] = {w0[f], row0[f], bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.segs, c.seg, c.block, c.fix, c.unit, x.t0, x.parts, f ? pl.share / 4 : pl.share, c.few, 0};
+            p.entries[e] = {w0[f], row0[f], bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.block, c.fix, c.unit, x.t0, x.parts, f ? pl.share / 4 : pl.share};
             w0[f] += c.unit * c.units;
-            row0[f] += c.rows * c.segs * a.pool.nkv;
+            row0[f] += c.rows * a.pool.nkv;
         }
     }
     __syncthreads();
@@ -279,22 +288,22 @@ __device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, con
     run -= 1;
     uint32_t e = run * pl.per;
     PaAt r;
-    r.x = lds.first[run];
+    r.x = pa_entry(p, pl.view, e);
     r.w0 = lds.w0[few][run];
     r.row0 = lds.row0[few][run];
     for (;;) {
-        r.c = pa_cut(p, r.x, pl.length);
+        r.c = pa_cut(p, r.x);
         const uint32_t n = r.c.few == (few != 0) ? r.c.unit * r.c.units : 0u;
         if (w - r.w0 < n || ++e >= E) break;
         r.w0 += n;
-        r.row0 += n ? r.c.rows * r.c.segs * a.pool.nkv : 0u;
-        r.x = pa_entry(p, e);
+        r.row0 += n ? r.c.rows * a.pool.nkv : 0u;
+        r.x = pa_entry(p, pl.view, e);
     }
     // the same for the whole wave: into scalar registers
     r.x.t0 = uniform(r.x.t0), r.x.tn = uniform(r.x.tn), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1), r.x.table = uniform(r.x.table);
     r.x.ps = uniform(r.x.ps), r.x.table0 = uniform(r.x.table0);
     r.x.parts = uniform(r.x.parts) != 0;
-    r.c = pa_cut(p, r.x, pl.length);
+    r.c = pa_cut(p, r.x);
     r.w0 = uniform(r.w0), r.row0 = uniform(r.row0);
     return r;
 }
@@ -326,23 +335,23 @@ __device__ __forceinline__ void pa_walk(const PaParams& p, const PaPlan& pl, con
     while (w < end) {
         const PaAt at = pa_find(p, pl, lds, few, w);
         const PaCut& c = at.c;
-        for (uint32_t u = (w - at.w0) / c.unit; u < c.units && w < end; u++) {
+        for (uint32_t u = pa_div(w - at.w0, c.unit); u < c.units && w < end; u++) {
             const uint32_t begin = at.w0 + u * c.unit, first = begin + c.fix;  // the first block's place
-            const uint32_t tile = u % c.tiles, seg = u / c.tiles % c.segs, n = min(c.seg, c.blocks - seg * c.seg);
+            const uint32_t kvh = c.tiles == 1 ? u : pa_div(u, c.tiles);
             // the blocks that begin in this share
-            const uint32_t i0 = w <= first ? 0u : (w - first + c.block - 1) / c.block;
-            const uint32_t i1 = min(n, end >= begin + c.unit ? n : end <= first ? 0u : (end - first + c.block - 1) / c.block);
+            const uint32_t i0 = w <= first ? 0u : pa_div(w - first + c.block - 1, c.block);
+            const uint32_t i1 = end >= begin + c.unit ? c.blocks : end <= first ? 0u : pa_div(end - first + c.block - 1, c.block);
             if (i0 < i1) {
                 PaItem it;
                 it.x = at.x;
                 it.rows = c.rows;
-                it.kvh = u / c.tiles / c.segs;
-                it.row0 = tile * c.tile;
-                it.b0 = seg * c.seg + i0;
-                it.b1 = seg * c.seg + i1;
+                it.kvh = uniform(kvh);
+                it.row0 = uniform((u - kvh * c.tiles) << c.tile);
+                it.b0 = uniform(i0);
+                it.b1 = uniform(i1);
                 it.shared = c.shared;
-                it.parts = at.x.parts || c.segs > 1 || i0 != 0 || i1 != n;
-                it.part = (size_t)at.row0 + (size_t)(u / c.tiles) * c.rows + it.row0 + (size_t)k * c.tile;
+                it.parts = at.x.parts || i0 != 0 || i1 != c.blocks;
+                it.part = (size_t)at.row0 + (size_t)it.kvh * c.rows + it.row0 + ((size_t)k << c.tile);
                 item(it);
             }
             w = begin + c.unit;
@@ -1035,7 +1044,7 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     // workgroup 8 i + x goes to XCD x
     const uint32_t half = PA_SHARES / 16, xcd = blockIdx.x % 8, slot = blockIdx.x / 8;
     const uint32_t k = (slot / half) * (PA_SHARES / 2) + xcd * half + slot % half;
-    const uint32_t w = k < pl.work / pl.share + 1 ? k * pl.share : pl.work, end = min(w + pl.share, pl.work);
+    const uint32_t w = k <= pa_div(pl.work, pl.share) ? k * pl.share : pl.work, end = min(w + pl.share, pl.work);
     pa_walk(p, pl, plan_lds, 0, w, min(end, pl.few0), k, [&](const PaItem& it) {
         if (HD == 256 || it.rows - it.row0 <= 64) pa_many_rows<HD, KVM, TERMS, 1>(p, it, plan_lds, st);
         else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2>(p, it, plan_lds, st);
@@ -1068,43 +1077,41 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
         const uint32_t r = found;
         if (r == 0xFFFFFFFFu) continue;
         const uint32_t kvh = min(h, a.nq - 1) / p.G;
-        // This row's parts of an entry: `n` places for them, not all in use.  Few rows: the shares that its unit's blocks lie in; many
-        // rows: two shares at most to a segment, whose blocks begin within one share's length.
-        struct Parts {
-            uint32_t n, row, first, k0;
-        };
-        auto parts = [&](const PaLeft& e) -> Parts {
+        // This row's parts of an entry: `n` of them, one in each share that its unit's blocks lie in, a tile apart.
+        auto parts = [&](const PaLeft& e, uint32_t& n) -> uint32_t {
             const uint32_t row = (t - e.t0) * p.G + h % p.G;
-            if (row >= e.rows) return {0, 0, 0, 0};  // (a request of no group)
-            const uint32_t first = e.w0 + (kvh * e.segs * e.tiles + row / e.tile) * e.unit + e.fix, k0 = first / e.per;
-            return {e.few ? (first + (e.blocks - 1) * e.block) / e.per - k0 + 1 : 2 * e.segs, row, first, k0};
-        };
-        auto place = [&](const PaLeft& e, const Parts& x, uint32_t i, bool& used) -> size_t {
-            if (e.few) return used = true, (size_t)e.row0 + kvh * e.rows + x.row + (size_t)(x.k0 + i) * e.tile;
-            const uint32_t seg = i / 2, first = x.first + seg * e.tiles * e.unit, k = first / e.per + i % 2;
-            used = i % 2 == 0 || (first + (min(e.seg, e.blocks - seg * e.seg) - 1) * e.block) / e.per == k;
-            return (size_t)e.row0 + (size_t)(kvh * e.segs + seg) * e.rows + x.row + (size_t)k * e.tile;
+            if (row >= e.rows) return n = 0u;  // (a request of no group)
+            const uint32_t first = e.w0 + (kvh * e.tiles + (row >> e.tile)) * e.unit + e.fix, k0 = pa_div(first, e.per);
+            n = pa_div(first + (e.blocks - 1) * e.block, e.per) - k0 + 1;
+            return e.row0 + kvh * e.rows + row + (k0 << e.tile);
         };
         const PaLeft rest = p.entries[a.n_groups + r];
-        PaLeft shared;
-        Parts x0 = {0, 0, 0, 0};
+        uint32_t n0 = 0, n1, at0 = 0, tile0 = 0;
         if (rest.parts) {
-            shared = p.entries[pa_group_of(a, r)];
-            x0 = parts(shared);
+            const PaLeft shared = p.entries[pa_group_of(a, a.d_cu_groups, r)];
+            at0 = parts(shared, n0);
+            tile0 = shared.tile;
         }
-        const Parts x1 = parts(rest);
-        uint32_t n = h < a.nq ? x0.n + x1.n : 0u;
-        if (!rest.parts && n) {  // written by the one that had it?
-            bool used = false;
-            if (rest.few ? n <= 1 : rest.segs == 1 && (place(rest, x1, 1, used), !used)) n = 0;
-        }
-        auto part = [&](uint32_t i, bool& used) -> size_t { return i < x0.n ? place(shared, x0, i, used) : place(rest, x1, i - x0.n, used); };
-        // a place to each lane: it works out where that is, and the row's lanes then read the places in use together
+        const uint32_t at1 = parts(rest, n1);
+        // (a row with one part was written by the share that had it)
+        const uint32_t n = h >= a.nq || (!rest.parts && n1 <= 1) ? 0u : n0 + n1;
+        // every lane reads one part's maximum and sum, then all read the parts' outputs together
         float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t i0 = group * L; i0 < n; i0 += L * GROUPS) {
-            bool used = false;
-            const uint32_t i = i0 + c, at = i < n ? (uint32_t)part(i, used) : 0u;
+            const uint32_t i = i0 + c, at = i < n0 ? at0 + (i << tile0) : at1 + ((i - n0) << rest.tile);
+            const bool used = i < n;
             const float2 v = used ? p.ml[at] : make_float2(-INFINITY, 0.f);
+            const uint32_t many = min(n - i0, L);
+            float4 x[4];
+            uint32_t u = 0;
+            auto four = [&]() {
+#pragma unroll
+                for (uint32_t k = 0; k < 4; k++) {
+                    const uint32_t from = (uint32_t)__shfl((int)at, min(u + k, L - 1), L);
+                    x[k] = u + k < many ? *reinterpret_cast<const float4*>(p.o + (size_t)from * HD + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
+                }
+            };
+            four();  // (on their way while the maximum is worked out)
             float top = v.x;
 #pragma unroll
             for (uint32_t d = 1; d < L; d *= 2) {
@@ -1119,22 +1126,15 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
             l = fmaf(l, by, sum);
 #pragma unroll
             for (int k = 0; k < 4; k++) o[k] *= by;
-            const unsigned long long all = __builtin_amdgcn_ballot_w64(used);
-            unsigned long long mine = L == 64 ? all : (all >> ((tid & 63u) / L * L)) & ((1ull << (L & 63)) - 1);
-            while (mine) {
-                float4 x[4];
-                float w4[4];
+            for (;;) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    const int lane = mine ? __builtin_ctzll(mine) : 0;
-                    w4[k] = mine ? __shfl(f, lane, L) : 0.f;
-                    const uint32_t from = (uint32_t)__shfl((int)at, lane, L);
-                    x[k] = mine ? *reinterpret_cast<const float4*>(p.o + (size_t)from * HD + 4 * c) : make_float4(0.f, 0.f, 0.f, 0.f);
-                    mine &= mine - 1;
+                for (uint32_t k = 0; k < 4; k++) {
+                    const float w = __shfl(f, min(u + k, L - 1), L), w4 = u + k < many ? w : 0.f;
+                    o[0] = fmaf(x[k].x, w4, o[0]), o[1] = fmaf(x[k].y, w4, o[1]), o[2] = fmaf(x[k].z, w4, o[2]), o[3] = fmaf(x[k].w, w4, o[3]);
                 }
-#pragma unroll
-                for (int k = 0; k < 4; k++)
-                    o[0] = fmaf(x[k].x, w4[k], o[0]), o[1] = fmaf(x[k].y, w4[k], o[1]), o[2] = fmaf(x[k].z, w4[k], o[2]), o[3] = fmaf(x[k].w, w4[k], o[3]);
+                u += 4;
+                if (u >= many) break;
+                four();
             }
         }
         if constexpr (GROUPS > 1) {
@@ -1166,10 +1166,9 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
 }
 
 // Rows of parts at most.  The part of unit u in share k begins u's rows and k tiles behind the first one of its kind: no two overlap,
-// because the next part is of the next unit or in the next share, and no unit has more rows than a tile.  Segments beyond an entry's first
-// stand for a share's work each, of which there are PA_SHARES.
+// because the next part is of the next unit or in the next share, and no unit has more rows than a tile.
 static uint64_t most_rows(const oxb_paged_attention& a) {
-    return (uint64_t)a.n_tokens * a.nq * (a.n_groups ? 2 : 1) + (uint64_t)PA_SHARES * (2 * pa_tile_many(a.pool.hd) + 4 * PA_TILE_FEW);
+    return (uint64_t)a.n_tokens * a.nq * (a.n_groups ? 2 : 1) + (uint64_t)PA_SHARES * (pa_tile_many(a.pool.hd) + (4u << PA_TILE_FEW_LOG));
 }
 static size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 static size_t entries_bytes(const oxb_paged_attention& a) { return up256(((size_t)a.n_groups + a.n_requests) * sizeof(PaLeft)); }
@@ -1208,8 +1207,8 @@ hipError_t oxb_launch_paged_attention(const oxb_paged_attention& a, hipStream_t 
     p.scale_log2 = (a.scale == 0.f ? 1.0f / sqrtf((float)a.pool.hd) : fabsf(a.scale)) * PA_LOG2E;
     p.negative = a.scale < 0.f ? 0x80000000u : 0u;
     p.page_shift = (uint32_t)__builtin_ctz(a.pool.page_size);
-    p.tile_many = pa_tile_many(a.pool.hd);
-    p.keys_many = pa_keys_many(a.pool.hd, a.pool.kv_dtype != OXB_KV_F16, a.dtype == OXB_DTYPE_F32);
+    p.tile_many_log = (uint32_t)__builtin_ctz(pa_tile_many(a.pool.hd));
+    p.keys_many_log = (uint32_t)__builtin_ctz(pa_keys_many(a.pool.hd, a.pool.kv_dtype != OXB_KV_F16, a.dtype == OXB_DTYPE_F32));
     p.cost = {1, 4, 3, 12};
     uint8_t* ws = reinterpret_cast<uint8_t*>(a.d_workspace);
     p.entries = reinterpret_cast<PaLeft*>(ws);
