@@ -33,7 +33,7 @@ typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 #define PA_TILE_FEW_LOG 4u
 #define PA_KEYS_FEW_LOG 5u // keys that such a wave takes at a time: 32
 #define PA_RUNS 256u       // runs of entries, one to a thread
-#define PA_STAGED 512u     // requests up to which a workgroup copies the lengths to LDS first
+#define PA_STAGED 256u     // requests up to which a workgroup copies the lengths to LDS first
 #define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk
 #define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes
 #define PA_LOG2E 1.44269504088896340736f
@@ -65,9 +65,8 @@ struct PaEntry {
     uint32_t t0, tn;    // queries
     uint32_t ps;        // keys 0 .. ps - 1 through the table row of the group's first request
     uint32_t k0, k1;    // and keys k0 .. k1 - 1 (k0 >= ps) through the own one
-    uint32_t table0, table;
-    bool parts;         // the rows have another part elsewhere
-    bool bad;           // sums that do not ascend
+    uint32_t table0;    // (its own one is table0 + own)
+    uint32_t own : 16, parts : 1, bad : 1;  // parts: the rows have another part elsewhere; bad: sums that do not ascend
 };
 
 // How an entry is cut.
@@ -130,12 +129,14 @@ __device__ __forceinline__ PaEntry pa_entry(const PaParams& p, const PaView& v, 
         r0 = g.r0;
         r1 = g.together ? g.r1 : r0;
         x.ps = x.k0 = x.k1 = g.prefix;
-        x.table0 = x.table = r0;
+        x.table0 = r0;
+        x.own = 0;
         x.parts = true;
     } else {
         r0 = e - a.n_groups;
         r1 = r0 + 1;
-        x.table0 = x.table = r0;
+        x.table0 = r0;
+        x.own = 0;
         x.ps = x.k0 = 0;
         x.parts = false;
         if (a.n_groups) {
@@ -145,6 +146,7 @@ __device__ __forceinline__ PaEntry pa_entry(const PaParams& p, const PaView& v, 
                 x.k0 = g.prefix;
                 x.ps = g.together ? 0u : g.prefix;
                 x.table0 = g.r0;
+                x.own = r0 - g.r0;
             }
         }
         x.bad = v.cu_tokens[r1] < v.cu_tokens[r0];
@@ -196,6 +198,7 @@ struct PaPlanLds {
     uint32_t work[2][4], rows[2][4], bad[4], most[4];
     uint32_t w0[2][PA_RUNS], row0[2][PA_RUNS];  // where the work and the rows of parts of a run begin: those of many rows, those of few
     int32_t cu_tokens[PA_STAGED + 1], lens[PA_STAGED], cu_groups[PA_STAGED + 1], prefix_lens[PA_STAGED];
+    PaEntry first[PA_RUNS];                     // a run's first entry
 };
 struct PaPlan {
     PaView view;
@@ -224,6 +227,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     for (uint32_t e = e0; e < e1; e++) {
         const PaEntry x = pa_entry(p, pl.view, e);
         const PaCut c = pa_cut(p, x);
+        if (e == e0) lds.first[tid] = x;
         bad |= x.bad;
         work[c.few] += c.unit * c.units;
         rows[c.few] += c.rows * a.pool.nkv;
@@ -260,7 +264,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
     if (bad) pl.work = 0;
     if (leave_entries) {
         for (uint32_t e = e0; e < e1; e++) {
-            const PaEntry x = pa_entry(p, pl.view, e);
+            const PaEntry x = e == e0 ? lds.first[tid] : pa_entry(p, pl.view, e);
             const PaCut c = pa_cut(p, x);
             const int f = c.few;
             p.entries[e] = {w0[f], row0[f], bad ? 0u : c.rows, c.tile, c.tiles, c.blocks, c.block, c.fix, c.unit, x.t0, x.parts, f ? pl.share / 4 : pl.share};
@@ -288,7 +292,7 @@ __device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, con
     run -= 1;
     uint32_t e = run * pl.per;
     PaAt r;
-    r.x = pa_entry(p, pl.view, e);
+    r.x = lds.first[run];
     r.w0 = lds.w0[few][run];
     r.row0 = lds.row0[few][run];
     for (;;) {
@@ -300,9 +304,8 @@ __device__ __forceinline__ PaAt pa_find(const PaParams& p, const PaPlan& pl, con
         r.x = pa_entry(p, pl.view, e);
     }
     // the same for the whole wave: into scalar registers
-    r.x.t0 = uniform(r.x.t0), r.x.tn = uniform(r.x.tn), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1), r.x.table = uniform(r.x.table);
-    r.x.ps = uniform(r.x.ps), r.x.table0 = uniform(r.x.table0);
-    r.x.parts = uniform(r.x.parts) != 0;
+    r.x.t0 = uniform(r.x.t0), r.x.tn = uniform(r.x.tn), r.x.ps = uniform(r.x.ps), r.x.k0 = uniform(r.x.k0), r.x.k1 = uniform(r.x.k1);
+    r.x.table0 = uniform(r.x.table0), r.x.own = uniform(r.x.own), r.x.parts = uniform(r.x.parts);
     r.c = pa_cut(p, r.x);
     r.w0 = uniform(r.w0), r.row0 = uniform(r.row0);
     return r;
@@ -322,7 +325,7 @@ struct PaSpan {
 };
 __device__ __forceinline__ PaSpan pa_span(const PaItem& it, uint32_t keys, uint32_t i) {
     const bool s = i < it.shared;
-    return {s ? i : it.x.k0 / keys + (i - it.shared), s ? 0u : it.x.k0, s ? it.x.ps : it.x.k1, s ? it.x.table0 : it.x.table};
+    return {s ? i : it.x.k0 / keys + (i - it.shared), s ? 0u : it.x.k0, s ? it.x.ps : it.x.k1, s ? it.x.table0 : it.x.table0 + it.x.own};
 }
 // Blocks in front of which all keys below `most` lie.
 __device__ __forceinline__ uint32_t pa_until(const PaItem& it, uint32_t keys, uint32_t most) {
