@@ -33,19 +33,21 @@ typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 #define PA_TILE_FEW_LOG 4u
 #define PA_KEYS_FEW_LOG 5u // keys that such a wave takes at a time: 32
 #define PA_RUNS 256u       // runs of entries, one to a thread
-#define PA_STAGED 256u     // requests up to which a workgroup copies the lengths to LDS first
+#define PA_STAGED 240u     // requests up to which a workgroup copies the lengths to LDS first
 #define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk
 #define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes
 #define PA_LOG2E 1.44269504088896340736f
 
-// Tiles of many rows and the keys of a block of theirs: what the registers and two workgroups' LDS hold.
+// Rows of a tile of many rows, and keys of a block of theirs, by what the registers and two workgroups' LDS hold.  Entries of up to 64
+// rows have one tile of 16 rows to a wave instead of two and take 64 keys whatever their type.
 constexpr uint32_t pa_tile_many(uint32_t hd) { return hd == 256 ? 64u : 128u; }
 constexpr uint32_t pa_keys_many(uint32_t hd, bool one_byte, bool two_terms) { return hd == 256 || one_byte || two_terms ? 32u : 64u; }
+constexpr uint32_t pa_keys_64(uint32_t hd) { return hd == 256 ? 32u : 64u; }
 
 // Work, in units that mean nothing but relative to each other: a block of 32 keys for few rows, a block for many rows, and
 // what a unit of either costs whatever its keys are.
 struct PaCosts {
-    uint32_t few, many, few_unit, many_unit;
+    uint32_t few, many, many_64_more, few_unit, many_unit;  // many_64_more: more for a block of an entry of up to 64 rows
 };
 
 struct PaParams {
@@ -54,7 +56,7 @@ struct PaParams {
     uint32_t negative; // the scale's sign bit, for q
     uint32_t G;        // q heads to a kv head
     uint32_t page_shift;
-    uint32_t tile_many_log, keys_many_log;
+    uint32_t tile_many_log, keys_many_log, keys_64_more;
     PaCosts cost;
     struct PaLeft* entries;  // workspace: what the merge needs of every entry
     float2* ml;        // maximum (log2 units) and sum of every part's rows
@@ -169,8 +171,9 @@ __device__ __forceinline__ PaCut pa_cut(const PaParams& p, const PaEntry& x) {
     c.rows = x.tn * p.G;
     c.few = c.rows <= PA_FEW;
     c.tile = c.few ? PA_TILE_FEW_LOG : p.tile_many_log;
-    c.keys = c.few ? PA_KEYS_FEW_LOG : p.keys_many_log;
-    c.block = c.few ? p.cost.few : p.cost.many;
+    const uint32_t some = c.rows <= 64 ? 1u : 0u;
+    c.keys = c.few ? PA_KEYS_FEW_LOG : p.keys_many_log + some * p.keys_64_more;
+    c.block = c.few ? p.cost.few : p.cost.many + some * p.cost.many_64_more;
     c.fix = c.few ? p.cost.few_unit : p.cost.many_unit;
     c.tiles = (c.rows + (1u << c.tile) - 1) >> c.tile;
     const uint32_t up = (1u << c.keys) - 1;
@@ -259,7 +262,7 @@ __device__ __forceinline__ PaPlan pa_plan(const PaParams& p, PaPlanLds& lds, boo
 #pragma unroll
     for (int f = 0; f < 2; f++) lds.w0[f][tid] = w0[f], lds.row0[f][tid] = row0[f];
     // four waves to a share, and no share without a block: parts are counted by the blocks that begin in a share
-    pl.share = max(((pl.work + PA_SHARES - 1) / PA_SHARES + 3) & ~3u, max(4 * p.cost.few, p.cost.many));
+    pl.share = max(((pl.work + PA_SHARES - 1) / PA_SHARES + 3) & ~3u, max(4 * p.cost.few, p.cost.many + p.cost.many_64_more));
     // (with sums that do not ascend the parts could pass the workspace: nothing is done at all)
     if (bad) pl.work = 0;
     if (leave_entries) {
@@ -685,10 +688,10 @@ struct PaStages {
     float* scales;
 };
 
-template <int HD, int KVM, int TERMS, int QT>
+template <int HD, int KVM, int TERMS, int QT, int KB>
 __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it, PaPlanLds& plan_lds, const PaStages& st) {
     constexpr bool QC = KVM != OXB_KV_F16;
-    constexpr int KB = (int)pa_keys_many(HD, KVM != OXB_KV_F16, TERMS == 2), KS = HD / 32, NS = HD / 16, NT = KB / 16, NH = KB / 32;
+    constexpr int KS = HD / 32, NS = HD / 16, NT = KB / 16, NH = KB / 32;
     constexpr uint32_t ROWB = HD * (QC ? 1 : 2);
     constexpr int PPR = HD / 8, RPW = KB / 4;                       // pieces of an LDS row; rows that a wave fetches
     constexpr int RB = PPR >= 16 ? 1 : 16 / PPR, PM = (PPR < 16 ? PPR : 16) - 1;  // rows of 256 bytes; the permutation's mask
@@ -1039,7 +1042,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 template <int HD, int KVM, int TERMS>
 __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel(PaParams p) {
     __shared__ PaPlanLds plan_lds;
-    constexpr int KB = (int)pa_keys_many(HD, KVM != OXB_KV_F16, TERMS == 2);
+    constexpr int KB = (int)pa_keys_64(HD);
     __shared__ __attribute__((aligned(16))) _Float16 k0[KB * HD], v0[KB * HD], k1[KB * HD], v1[KB * HD];
     __shared__ __attribute__((aligned(16))) float scales[4 * KB];
     const PaStages st = {k0, v0, k1, v1, scales};
@@ -1049,8 +1052,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
     const uint32_t k = (slot / half) * (PA_SHARES / 2) + xcd * half + slot % half;
     const uint32_t w = k <= pa_div(pl.work, pl.share) ? k * pl.share : pl.work, end = min(w + pl.share, pl.work);
     pa_walk(p, pl, plan_lds, 0, w, min(end, pl.few0), k, [&](const PaItem& it) {
-        if (HD == 256 || it.rows - it.row0 <= 64) pa_many_rows<HD, KVM, TERMS, 1>(p, it, plan_lds, st);
-        else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2>(p, it, plan_lds, st);
+        if (HD == 256 || it.rows <= 64) pa_many_rows<HD, KVM, TERMS, 1, (int)pa_keys_64(HD)>(p, it, plan_lds, st);
+        else if constexpr (HD < 256) pa_many_rows<HD, KVM, TERMS, 2, (int)pa_keys_many(HD, KVM != OXB_KV_F16, TERMS == 2)>(p, it, plan_lds, st);
     });
     const uint32_t wave = uniform(threadIdx.x >> 6), quarter = pl.share / 4, from = w + wave * quarter;
     pa_walk(p, pl, plan_lds, 1, max(from, pl.few0), min(from + quarter, end), 4 * k + wave, [&](const PaItem& it) { pa_few_rows<HD, KVM, TERMS>(p, it); });
@@ -1212,7 +1215,8 @@ hipError_t oxb_launch_paged_attention(const oxb_paged_attention& a, hipStream_t 
     p.page_shift = (uint32_t)__builtin_ctz(a.pool.page_size);
     p.tile_many_log = (uint32_t)__builtin_ctz(pa_tile_many(a.pool.hd));
     p.keys_many_log = (uint32_t)__builtin_ctz(pa_keys_many(a.pool.hd, a.pool.kv_dtype != OXB_KV_F16, a.dtype == OXB_DTYPE_F32));
-    p.cost = {1, 4, 3, 12};
+    p.keys_64_more = (uint32_t)__builtin_ctz(pa_keys_64(a.pool.hd)) - p.keys_many_log;
+    p.cost = {1, 4, 0, 3, 12};
     uint8_t* ws = reinterpret_cast<uint8_t*>(a.d_workspace);
     p.entries = reinterpret_cast<PaLeft*>(ws);
     ws += entries_bytes(a);
