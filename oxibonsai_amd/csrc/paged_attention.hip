@@ -405,7 +405,9 @@ __device__ __forceinline__ float pa_lse(float m, float l) { return l > 0.f ? (m 
 
 // ---------------------------------------------------------------------------
 // Few rows: a request's rest, a small group's prefix.  A wave has 16 rows and shares nothing with the others; operands come from
-// memory straight into registers, the next block of 32 keys while this one is worked on.
+// memory straight into registers, 16 KB for 32 keys (head_dim 128, fp16).  Bound by memory: the eight waves of a CU have 64 to 128 KB on their
+// way, which is enough (a second block on its way to every wave: 62 requests 42.9 us instead of 40.4, the call).  fp16 rows, which are
+// read once, are not kept in the caches: 256 requests 166 us -> 159 (one-byte rows 40.5 -> 42.0, so they are).
 //
 // Products as in the prefill attention, transposed, on v_mfma_f32_16x16x32_f16: S^T = K Q^T leaves a lane (row c = lane % 16,
 // g = lane / 16) the scores of keys 4 g .. and 16 + 4 g .. of a block, which is where O^T = V^T P^T wants its probabilities.  V as
@@ -429,12 +431,14 @@ struct PaBlock {
     v4f ks[2], vs[2];
 };
 
-template <int N>
+// N dwords; ONCE: they are not kept in the caches (what a request reads alone makes room for the prefix, which others read too).
+template <bool ONCE, int N>
 __device__ __forceinline__ void pa_read(uint32_t (&d)[N], const uint8_t* p) {
     if constexpr (N >= 4) {
 #pragma unroll
         for (int i = 0; i < N / 4; i++) {
-            const v4w w = *reinterpret_cast<const v4w*>(p + 16 * i);
+            const v4w* q = reinterpret_cast<const v4w*>(p + 16 * i);
+            const v4w w = ONCE ? __builtin_nontemporal_load(q) : *q;
             d[4 * i] = w.x, d[4 * i + 1] = w.y, d[4 * i + 2] = w.z, d[4 * i + 3] = w.w;
         }
     } else if constexpr (N == 2) {
@@ -482,11 +486,11 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
             const uint8_t *kr = Kc + r * ROWB, *vr = Vc + r * ROWB;
             const uint32_t kc = max(min(c, to), from) * ROWB;
 #pragma unroll
-            for (int s = 0; s < Block::KW; s++) pa_read(B.k[kt][s], kr + kc + (QC ? (KS > 1 ? 64u * s + 16u * g : 8u * g) : 64u * s + 16u * g));
+            for (int s = 0; s < Block::KW; s++) pa_read<!QC>(B.k[kt][s], kr + kc + (QC ? (KS > 1 ? 64u * s + 16u * g : 8u * g) : 64u * s + 16u * g));
 #pragma unroll
             for (uint32_t e = 0; e < 4; e++) {
                 const uint8_t* vp = vr + max(min(4 * g + e, to), from) * ROWB + c * (DPL * (QC ? 1 : 2));
-                if constexpr (DPL * (QC ? 1 : 2) >= 4) pa_read(B.v[4 * kt + e], vp);
+                if constexpr (DPL * (QC ? 1 : 2) >= 4) pa_read<!QC>(B.v[4 * kt + e], vp);
                 else B.v[4 * kt + e][0] = *reinterpret_cast<const uint16_t*>(vp);
             }
             if constexpr (QC) {
@@ -495,10 +499,8 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
             }
         }
     };
-    // (two blocks of wide rows do not fit the registers)
-    constexpr bool AHEAD = HD < 256;
     const bool any = it.x.ps > 0 || it.x.k1 > it.x.k0;
-    Block A, B;
+    Block A;
     if (any) request(A, it.b0);
 
     v8h q[TERMS][KS];
@@ -629,19 +631,9 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
             for (int t = 0; t < TERMS; t++) O[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(V, P[t], O[j], 0, 0, 0);
         }
     };
-    if constexpr (AHEAD) {
-        for (uint32_t b = it.b0; b < b1; b += 2) {
-            if (b + 1 < b1) request(B, b + 1);
-            block(A, b);
-            if (b + 1 >= b1) break;
-            if (b + 2 < b1) request(A, b + 2);
-            block(B, b + 1);
-        }
-    } else {
-        for (uint32_t b = it.b0; b < b1; b++) {
-            if (b > it.b0) request(A, b);
-            block(A, b);
-        }
+    for (uint32_t b = it.b0; b < b1; b++) {
+        if (b > it.b0) request(A, b);
+        block(A, b);
     }
     l = sum_rows4(l);
     if (!there) return;
@@ -873,6 +865,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             }
         };
         v4f S[QT][NT];
+        __builtin_amdgcn_s_setprio(1);  // (the products first, where another wave of the SIMD is at its softmax)
 #pragma unroll
         for (int s = 0; s < KS; s++) read_k(0, s);
         fence();
@@ -896,6 +889,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
                 }
             }
         read_v(0);
+        __builtin_amdgcn_s_setprio(0);
         fence();
         const bool all = key0 >= sp.lo && key0 + KB <= min(least, sp.hi);  // (wave-uniform) every row sees all of these keys
         v8h P[TERMS][QT][NH];
