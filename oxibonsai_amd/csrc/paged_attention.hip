@@ -680,6 +680,10 @@ struct PaStages {
     float* scales;
 };
 
+// A CU's second workgroup goes a step above its first, which the hardware prefers as the older one (a prompt chunk's second halves ended
+// a fifth later).
+#define pa_priority(n) (blockIdx.x >= PA_SHARES / 2 ? __builtin_amdgcn_s_setprio((n) + 1) : __builtin_amdgcn_s_setprio(n))
+
 template <int HD, int KVM, int TERMS, int QT, int KB>
 __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it, PaPlanLds& plan_lds, const PaStages& st) {
     constexpr bool QC = KVM != OXB_KV_F16;
@@ -865,7 +869,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             }
         };
         v4f S[QT][NT];
-        __builtin_amdgcn_s_setprio(1);  // (the products first, where another wave of the SIMD is at its softmax)
+        pa_priority(1);  // (the products first, where another wave of the SIMD is at its softmax)
 #pragma unroll
         for (int s = 0; s < KS; s++) read_k(0, s);
         fence();
@@ -889,7 +893,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
                 }
             }
         read_v(0);
-        __builtin_amdgcn_s_setprio(0);
+        pa_priority(0);
         fence();
         const bool all = key0 >= sp.lo && key0 + KB <= min(least, sp.hi);  // (wave-uniform) every row sees all of these keys
         v8h P[TERMS][QT][NH];

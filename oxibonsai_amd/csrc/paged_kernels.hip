@@ -15,8 +15,8 @@
 // With held = ceil(kept / P), had = ceil(past / P), has = ceil((kept + add) / P) of each request, the exclusive sums of had - held,
 // has - held and add over the requests give every freed page its place on the stack of free pages, every new page the entry it
 // comes from and every token its row.  One workgroup works the sums out (the numbers of a step fit its LDS: 4096 requests are
-// two arrays of 16 KB) and moves the freed pages; the tokens' slots follow in the same launch while they are few, else in a
-// second one over the whole chip.  Latency bound: three dependent reads, two scans.
+// three arrays of 16 KB) and moves the freed pages; the tokens' slots follow in the same launch while they are few, else in a
+// second one over the whole chip.  Latency bound: a trip to memory for the lengths, one for a page given up, one for a table entry.
 // ---------------------------------------------------------------------------
 #define PAGES_THREADS 1024
 #define PAGES_ROWS_PER_WG 1024     // of the second launch
@@ -33,121 +33,173 @@ __device__ __forceinline__ uint32_t pages_find(const int* cu, uint32_t n, int i)
     return lo;
 }
 
+// Copies in LDS of what a step's rows need of its requests, [n_requests + 1] each.
+struct PagesLds {
+    int *cu_tokens, *lens, *cu_pages;
+};
+__device__ __forceinline__ PagesLds pages_lds(int* lds, uint32_t B) { return {lds, lds + B + 1, lds + 2 * (B + 1)}; }
+
 // Row i: its token's position and slot; the token that opens a new page also enters it into the table.  `top`: free pages before
 // the new ones were taken.
-__device__ __forceinline__ void pages_row(const oxb_page_assign& a, uint32_t i, const int* cu_tokens, int top) {
+__device__ __forceinline__ void pages_row(const oxb_page_assign& a, uint32_t i, const PagesLds& l, int top, uint32_t shift) {
     int slot = -1, pos = -1;
-    if ((int)i < cu_tokens[a.n_requests]) {
-        const uint32_t r = pages_find(cu_tokens, a.n_requests, (int)i);
-        const int first = cu_tokens[r], add = cu_tokens[r + 1] - first, P = (int)a.page_size;
-        const int kept = a.d_lens[r] - add, held = (kept + P - 1) / P;
+    if ((int)i < l.cu_tokens[a.n_requests]) {
+        const uint32_t r = pages_find(l.cu_tokens, a.n_requests, (int)i);
+        const int first = l.cu_tokens[r], add = l.cu_tokens[r + 1] - first, P = 1 << shift;
+        const int kept = l.lens[r] - add, held = (kept + P - 1) >> shift;
         pos = kept + (int)i - first;
-        const int at = pos / P, off = pos % P;
+        const int at = pos >> shift, off = pos & (P - 1);
         int* entry = a.d_tables + (size_t)r * a.table_width + at;
         int page;
         if (at >= held) {
-            page = a.d_free_pages[top - 1 - (a.d_cu_pages[r] + at - held)];
+            page = a.d_free_pages[top - 1 - (l.cu_pages[r] + at - held)];
             if (off == 0) *entry = page;
         } else {
             page = *entry;
         }
-        if ((uint32_t)page < a.n_pages) slot = page * P + off;
+        if ((uint32_t)page < a.n_pages) slot = (page << shift) + off;
     }
     a.d_slots[i] = slot;
     a.d_positions[i] = pos;
 }
 
-struct PagesSum {
-    long long freed, need, add;
-};
-__device__ __forceinline__ PagesSum pages_plus(const PagesSum& x, const PagesSum& y) { return {x.freed + y.freed, x.need + y.need, x.add + y.add}; }
+// Inclusive sum over the 64 lanes of a wave: four steps inside rows of 16 lanes, then the rows' last lanes to the rows behind them.
+__device__ __forceinline__ uint32_t pages_scan(uint32_t v) {
+    v += dpp_u32<OXB_DPP_ROW_SHR(1)>(v);
+    v += dpp_u32<OXB_DPP_ROW_SHR(2)>(v);
+    v += dpp_u32<OXB_DPP_ROW_SHR(4)>(v);
+    v += dpp_u32<OXB_DPP_ROW_SHR(8)>(v);
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15
+    v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31
+    return v;
+}
 
-__global__ __launch_bounds__(PAGES_THREADS) void pages_assign_kernel(oxb_page_assign a, uint32_t rows_here) {
-    extern __shared__ int pages_lds[];  // [n_requests + 1] sums of the freed pages, then as many of the new tokens
+// Sums of a run of requests.  Their 32 bits hold what a call that succeeds can add up to; whether one has passed them is told by
+// the sums as floats.
+struct PagesSum {
+    uint32_t freed, need, add;
+};
+__global__ __launch_bounds__(PAGES_THREADS) void pages_assign_kernel(oxb_page_assign a, uint32_t rows_here, uint32_t shift) {
+    extern __shared__ int lds[];
     __shared__ PagesSum wave_sum[PAGES_THREADS / 64];
-    __shared__ int bad[2];              // a length that is none; a table row that is too short
+    __shared__ float wave_size[PAGES_THREADS / 64][3];
+    __shared__ uint32_t wave_bad[PAGES_THREADS / 64];  // 1: a length that is none; 2: a table row that is too short
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, B = a.n_requests;
-    int* const cu_freed = pages_lds;
-    int* const cu_tokens = pages_lds + B + 1;
-    const int P = (int)a.page_size, n_free = *a.d_n_free;
-    if (tid < 2) bad[tid] = 0;
-    __syncthreads();
+    const PagesLds l = pages_lds(lds, B);
+    int* const cu_freed = l.cu_pages;  // (until the freed pages are where they go)
+    const int P = 1 << shift, n_free = *a.d_n_free;
     const uint32_t per = (B + PAGES_THREADS - 1) / PAGES_THREADS, r0 = min(tid * per, B), r1 = min(r0 + per, B);
+    auto pages = [&](int n) -> uint32_t { return ((uint32_t)n + P - 1) >> shift; };
     auto look = [&](uint32_t r, int& kept, int& past, int& add) {
         past = a.d_past[r];
         add = a.d_add[r];
         kept = a.d_keep ? min(a.d_keep[r], past) : past;
     };
-    // (a length that is none or passes the table counts as 0: the call fails, and no sum overflows)
-    auto count = [&](uint32_t r, PagesSum& s) {
-        int kept, past, add;
-        look(r, kept, past, add);
-        const long long width = (long long)a.table_width * P;
-        if (kept < 0 || past < 0 || add < 0) bad[0] = 1;
-        else if ((long long)kept + add > width || past > width) bad[1] = 1;
-        else s = pages_plus(s, {(past + P - 1) / P - (kept + P - 1) / P, (kept + add + P - 1) / P - (kept + P - 1) / P, add});
+    // (a length that is none or passes the table counts as 0: the call fails)
+    auto count = [&](int kept, int past, int add, PagesSum& s) -> uint32_t {
+        const uint32_t width = a.table_width << shift;  // (below 2^31)
+        if (kept < 0 || past < 0 || add < 0) return 1u;
+        if ((uint32_t)kept + (uint32_t)add > width || (uint32_t)past > width) return 2u;
+        s.freed += pages(past) - pages(kept);
+        s.need += pages(kept + add) - pages(kept);
+        s.add += add;
+        return 0u;
     };
     PagesSum mine = {0, 0, 0};
-    for (uint32_t r = r0; r < r1; r++) count(r, mine);
-    // exclusive sums over the threads
-    PagesSum incl = mine;
+    float size[3] = {0.f, 0.f, 0.f};
+    uint32_t bad = 0;
+    int kept = 0, past = 0, add = 0;
+    for (uint32_t r = r0; r < r1; r++) {
+        PagesSum one = {0, 0, 0};
+        look(r, kept, past, add);
+        bad |= count(kept, past, add, one);
+        mine = {mine.freed + one.freed, mine.need + one.need, mine.add + one.add};
+        size[0] += (float)one.freed, size[1] += (float)one.need, size[2] += (float)one.add;
+    }
+    const PagesSum incl = {pages_scan(mine.freed), pages_scan(mine.need), pages_scan(mine.add)};
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const PagesSum o = {__shfl_up(incl.freed, d, 64), __shfl_up(incl.need, d, 64), __shfl_up(incl.add, d, 64)};
-        if (lane >= (uint32_t)d) incl = pages_plus(incl, o);
+    for (int i = 0; i < 3; i++) size[i] = wave_sum_f32(size[i]);
+    bad = (__builtin_amdgcn_ballot_w64(bad & 1u) ? 1u : 0u) | (__builtin_amdgcn_ballot_w64(bad & 2u) ? 2u : 0u);
+    if (lane == 63) {
+        wave_sum[wave] = incl;
+        wave_bad[wave] = bad;
+#pragma unroll
+        for (int i = 0; i < 3; i++) wave_size[wave][i] = size[i];
     }
-    if (lane == 63) wave_sum[wave] = incl;
     __syncthreads();
-    PagesSum before = {0, 0, 0}, total = {0, 0, 0};
+    PagesSum before = {incl.freed - mine.freed, incl.need - mine.need, incl.add - mine.add}, total = {0, 0, 0};
+    size[0] = size[1] = size[2] = 0.f;
+#pragma unroll
     for (uint32_t w = 0; w < PAGES_THREADS / 64; w++) {
-        if (w < wave) before = pages_plus(before, wave_sum[w]);
-        total = pages_plus(total, wave_sum[w]);
+        const PagesSum s = wave_sum[w];
+        if (w < wave) before = {before.freed + s.freed, before.need + s.need, before.add + s.add};
+        total = {total.freed + s.freed, total.need + s.need, total.add + s.add};
+        bad |= wave_bad[w];
+#pragma unroll
+        for (int i = 0; i < 3; i++) size[i] += wave_size[w][i];
     }
-    const bool wrong = bad[0] || n_free < 0 || n_free + total.freed > (long long)a.n_pages;
-    const int status = wrong ? 3 : total.need > n_free + total.freed ? 1 : bad[1] || total.add > (long long)a.n_rows ? 2 : 0;
+    const float most = 2147483648.f;
+    const bool wrong = (bad & 1u) || n_free < 0 || size[0] >= most || (uint32_t)n_free + total.freed > a.n_pages;
+    const int status = wrong ? 3 : size[1] >= most || total.need > (uint32_t)n_free + total.freed ? 1 : (bad & 2u) || size[2] >= most || total.add > a.n_rows ? 2 : 0;
     const bool ok = status == 0;
+    const int top = n_free + (ok ? (int)total.freed : 0);
     if (tid == 0) {
         a.d_status[0] = status;
-        a.d_status[1] = (int)min(total.need, 0x7FFFFFFFll);
-        *a.d_n_free_out = ok ? (int)(n_free + total.freed - total.need) : n_free;  // (every thread has read n_free: two barriers ago)
-        cu_freed[0] = cu_tokens[0] = a.d_cu_tokens[0] = a.d_cu_pages[0] = 0;
+        a.d_status[1] = size[1] >= most ? 0x7FFFFFFF : (int)total.need;
+        *a.d_n_free_out = ok ? top - (int)total.need : n_free;  // (every thread has read n_free: a barrier ago)
+        cu_freed[0] = l.cu_tokens[0] = a.d_cu_tokens[0] = a.d_cu_pages[0] = 0;
     }
-    PagesSum at = {before.freed + incl.freed - mine.freed, before.need + incl.need - mine.need, before.add + incl.add - mine.add};
+    PagesSum at = before;
     for (uint32_t r = r0; r < r1; r++) {
-        int kept, past, add;
-        look(r, kept, past, add);
-        if (ok) count(r, at);
-        a.d_lens[r] = ok ? kept + add : past;
-        a.d_cu_tokens[r + 1] = cu_tokens[r + 1] = ok ? (int)at.add : 0;
+        if (per > 1) look(r, kept, past, add);
+        if (ok) count(kept, past, add, at);
+        a.d_lens[r] = l.lens[r] = ok ? kept + add : past;
+        a.d_cu_tokens[r + 1] = l.cu_tokens[r + 1] = ok ? (int)at.add : 0;
         a.d_cu_pages[r + 1] = ok ? (int)at.need : 0;
         cu_freed[r + 1] = ok ? (int)at.freed : 0;
     }
     __syncthreads();
     // pages given up: page i of them goes to place n_free + i of the stack
-    for (int i = (int)tid; i < cu_freed[B]; i += PAGES_THREADS) {
-        const uint32_t r = pages_find(cu_freed, B, i);
-        const int kept = a.d_lens[r] - (cu_tokens[r + 1] - cu_tokens[r]), held = (kept + P - 1) / P;
-        a.d_free_pages[n_free + i] = a.d_tables[(size_t)r * a.table_width + held + i - cu_freed[r]];
+    if (ok)
+        for (int i = (int)tid; i < (int)total.freed; i += PAGES_THREADS) {
+            const uint32_t r = pages_find(cu_freed, B, i);
+            const int held = (int)pages(l.lens[r] - (l.cu_tokens[r + 1] - l.cu_tokens[r]));
+            a.d_free_pages[n_free + i] = a.d_tables[(size_t)r * a.table_width + held + i - cu_freed[r]];
+        }
+    if (rows_here == 0) return;
+    __syncthreads();
+    at = before;
+    if (tid == 0) l.cu_pages[0] = 0;
+    for (uint32_t r = r0; r < r1; r++) {
+        if (per > 1) kept = l.lens[r] - (l.cu_tokens[r + 1] - l.cu_tokens[r]), add = l.cu_tokens[r + 1] - l.cu_tokens[r];
+        if (ok) at.need += pages(kept + add) - pages(kept);
+        l.cu_pages[r + 1] = ok ? (int)at.need : 0;
     }
     __syncthreads();
-    for (uint32_t i = tid; i < rows_here; i += PAGES_THREADS) pages_row(a, i, cu_tokens, n_free + cu_freed[B]);
+    for (uint32_t i = tid; i < rows_here; i += PAGES_THREADS) pages_row(a, i, l, top, shift);
 }
 
-__global__ __launch_bounds__(256) void pages_rows_kernel(oxb_page_assign a) {
-    extern __shared__ int pages_lds[];  // [n_requests + 1] sums of the new tokens
+__global__ __launch_bounds__(256) void pages_rows_kernel(oxb_page_assign a, uint32_t shift) {
+    extern __shared__ int lds[];
     const uint32_t B = a.n_requests, i0 = blockIdx.x * PAGES_ROWS_PER_WG;
-    for (uint32_t r = threadIdx.x; r <= B; r += 256) pages_lds[r] = a.d_cu_tokens[r];
+    const PagesLds l = pages_lds(lds, B);
+    for (uint32_t r = threadIdx.x; r <= B; r += 256) {
+        l.cu_tokens[r] = a.d_cu_tokens[r];
+        l.cu_pages[r] = a.d_cu_pages[r];
+        if (r < B) l.lens[r] = a.d_lens[r];
+    }
     const int top = *a.d_n_free_out + a.d_cu_pages[B];
     __syncthreads();
-    for (uint32_t i = i0 + threadIdx.x; i < min(i0 + PAGES_ROWS_PER_WG, a.n_rows); i += 256) pages_row(a, i, pages_lds, top);
+    for (uint32_t i = i0 + threadIdx.x; i < min(i0 + PAGES_ROWS_PER_WG, a.n_rows); i += 256) pages_row(a, i, l, top, shift);
 }
 
 hipError_t oxb_launch_paged_assign(const oxb_page_assign& a, hipStream_t st) {
-    const uint32_t here = a.n_rows <= PAGES_ROWS_AT_ONCE ? a.n_rows : 0;
-    hipLaunchKernelGGL(pages_assign_kernel, dim3(1), dim3(PAGES_THREADS), 2 * (a.n_requests + 1) * sizeof(int), st, a, here);
+    const uint32_t here = a.n_rows <= PAGES_ROWS_AT_ONCE ? a.n_rows : 0, shift = (uint32_t)__builtin_ctz(a.page_size);
+    const size_t lds = 3 * (a.n_requests + 1) * sizeof(int);
+    hipLaunchKernelGGL(pages_assign_kernel, dim3(1), dim3(PAGES_THREADS), lds, st, a, here, shift);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || here == a.n_rows) return e;
-    hipLaunchKernelGGL(pages_rows_kernel, dim3((a.n_rows + PAGES_ROWS_PER_WG - 1) / PAGES_ROWS_PER_WG), dim3(256), (a.n_requests + 1) * sizeof(int), st, a);
+    hipLaunchKernelGGL(pages_rows_kernel, dim3((a.n_rows + PAGES_ROWS_PER_WG - 1) / PAGES_ROWS_PER_WG), dim3(256), lds, st, a, shift);
     return hipGetLastError();
 }
 
