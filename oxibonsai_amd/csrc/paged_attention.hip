@@ -400,6 +400,10 @@ __device__ __forceinline__ void pa_store4(void* out, uint32_t dtype, size_t at, 
         *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) =
             make_uint2(pa_bits16(v[0], dtype) | pa_bits16(v[1], dtype) << 16, pa_bits16(v[2], dtype) | pa_bits16(v[3], dtype) << 16);
 }
+// The exponent of a value row's scale, -100 .. 100: a smaller one counts as 2^-100, so that no probability relative to it overflows; a
+// larger one, or none, as 2^100, so that the sum of the probabilities does not vanish beside it (fp16 probabilities that overflow
+// for it make outputs that are not finite, and the row is done again).
+__device__ __forceinline__ float pa_exponent(float scale) { return (float)((int)(min(max(__float_as_uint(scale) & 0x7FFFFFFFu, 27u << 23), 227u << 23) >> 23) - 127); }
 // Natural logarithm of the sum from its maximum in log2 units.
 __device__ __forceinline__ float pa_lse(float m, float l) { return l > 0.f ? (m + log2f(l)) * 0.693147180559945309417f : l == 0.f ? -INFINITY : NAN; }
 
@@ -574,8 +578,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
                     if constexpr (QC) vs[kt][v] = seen ? vs[kt][v] : 1.f;
                 }
                 S[kt][v] = s;
-                // (a scale below 2^-100 counts as that, so that no probability relative to it overflows)
-                if constexpr (QC) s += (float)((int)(max(__float_as_uint(vs[kt][v]) & 0x7FFFFFFFu, 27u << 23) >> 23) - 127);
+                if constexpr (QC) s += pa_exponent(vs[kt][v]);
                 top = fmaxf(top, s);
             }
         top = max_rows4(top);
@@ -636,6 +639,10 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
         block(A, b);
     }
     l = sum_rows4(l);
+    float odd = 0.f;  // no number, or infinite, if one of the row's outputs is
+#pragma unroll
+    for (int j = 0; j < DPL; j++) odd += O[j][0] + O[j][1] + O[j][2] + O[j][3];
+    odd = sum_rows4(odd);
     if (!there) return;
     const size_t part = it.part + c;
     const float inv = it.parts ? 1.f : l == 0.f ? 0.f : 1.0f / l;
@@ -658,8 +665,8 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
         }
     }
     if (g == 0) {
-        if (it.parts) p.ml[part] = make_float2(m, l);
-        else if (a.d_lse) a.d_lse[(size_t)tok * a.nq + head] = pa_lse(m, l);
+        p.ml[part] = make_float2(it.parts ? m : odd, l);
+        if (!it.parts && a.d_lse) a.d_lse[(size_t)tok * a.nq + head] = pa_lse(m, l);
     }
 }
 
@@ -931,7 +938,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 #pragma unroll
             for (int v = 0; v < 4; v++) {
                 float e = 0.f;
-                if constexpr (QC) e = (float)((int)(max(__float_as_uint(vs[kt][v]) & 0x7FFFFFFFu, 27u << 23) >> 23) - 127);
+                if constexpr (QC) e = pa_exponent(vs[kt][v]);
 #pragma unroll
                 for (int t = 0; t < QT; t++) top[t] = fmaxf(top[t], QC ? fmaf(S[t][kt][v], mul[t], e) : S[t][kt][v]);
             }
@@ -1021,6 +1028,10 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 #pragma unroll
     for (int t = 0; t < QT; t++) {
         const float sum = sum_rows4(l[t]);
+        float odd = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; i++) odd += O[t][i][0] + O[t][i][1] + O[t][i][2] + O[t][i][3];
+        odd = sum_rows4(odd);
         if (!there[t]) continue;
         const size_t part = it.part + (t * 4 + wave) * 16 + c;
         const float inv = it.parts ? 1.f : sum == 0.f ? 0.f : 1.0f / sum;
@@ -1031,8 +1042,8 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
             else pa_store4(a.d_out, a.dtype, (size_t)tok[t] * a.out_stride + (size_t)head[t] * HD + 16 * i + 4 * g, o);
         }
         if (g == 0) {
-            if (it.parts) p.ml[part] = make_float2(m[t], sum);
-            else if (a.d_lse) a.d_lse[(size_t)tok[t] * a.nq + head[t]] = pa_lse(m[t], sum);
+            p.ml[part] = make_float2(it.parts ? m[t] : odd, sum);
+            if (!it.parts && a.d_lse) a.d_lse[(size_t)tok[t] * a.nq + head[t]] = pa_lse(m[t], sum);
         }
     }
 }
@@ -1058,6 +1069,68 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 }
 
 // ---------------------------------------------------------------------------
+// A row over again, key by key and only the keys that it sees, by HD / 4 lanes.  The products of a block that only some of its rows see
+// multiply the values of a key that a row does not see by 0, which is no number where that value, or its row's scale, is infinite or
+// none itself: such rows, a finite sum of probabilities beside an output that is not finite, come here.  Slow (a key at a time, about
+// 1 us each) and rare; with infinities that the row does see the answer is the same as before.
+// ---------------------------------------------------------------------------
+template <int HD>
+__device__ __forceinline__ void pa_row_again(const PaParams& p, uint32_t r, uint32_t t, uint32_t h, uint32_t c, float o[4]) {
+    constexpr uint32_t L = HD / 4;
+    const oxb_paged_attention& a = p.a;
+    const PaView view = {a.d_cu_tokens, a.d_lens, a.d_cu_groups, a.d_prefix_lens};
+    const PaEntry x = pa_entry(p, view, a.n_groups + r);
+    const int pos = a.d_positions[t];
+    const uint32_t sees = pa_clamp(pos, 0x7FFFFFFEu) + (pos >= 0 ? 1u : 0u), end = min(max(x.k0, x.k1), sees);
+    const size_t at_q = (size_t)t * a.q_stride + (size_t)h * HD + 4 * c;
+    float q[4], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const float v = a.dtype == OXB_DTYPE_F32 ? reinterpret_cast<const float*>(a.d_q)[at_q + j]
+                        : a.dtype == OXB_DTYPE_F16 ? (float)reinterpret_cast<const _Float16*>(a.d_q)[at_q + j] : __uint_as_float((uint32_t)reinterpret_cast<const uint16_t*>(a.d_q)[at_q + j] << 16);
+        q[j] = __uint_as_float(__float_as_uint(v) ^ p.negative);
+        o[j] = 0.f;
+    }
+    auto values = [&](const void* rows, const float* scales, size_t row, float v[4]) {
+        const size_t at = row * HD + 4 * c;
+        uint32_t d[2];
+        if (a.pool.kv_dtype == OXB_KV_F16) {
+            const uint2 w = *reinterpret_cast<const uint2*>(reinterpret_cast<const _Float16*>(rows) + at);
+            d[0] = w.x, d[1] = w.y;
+        } else {
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint8_t*>(rows) + at);
+            if (a.pool.kv_dtype == OXB_KV_I8) kv_dec4<OXB_KV_I8>(w, d[0], d[1]);
+            else kv_dec4<OXB_KV_FP8_E4M3>(w, d[0], d[1]);
+        }
+        const float s = a.pool.kv_dtype == OXB_KV_F16 ? 1.f : scales[row];
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = (float)__builtin_bit_cast(_Float16, (uint16_t)(d[j / 2] >> (j % 2 * 16))) * s;
+    };
+#pragma unroll 1
+    for (uint32_t key = 0; key < end; key++) {
+        const uint32_t table = x.table0 + (key < x.k0 ? 0u : x.own);
+        const uint32_t page = min((uint32_t)a.d_tables[(size_t)table * a.table_width + (key >> p.page_shift)], a.pool.n_pages - 1);
+        const size_t row = (((size_t)(h / p.G) * a.pool.n_pages + page) << p.page_shift) + (key & (a.pool.page_size - 1u));
+        float k[4], v[4], s = 0.f;
+        values(a.pool.d_k, a.pool.d_k_scale, row, k);
+        values(a.pool.d_v, a.pool.d_v_scale, row, v);
+#pragma unroll
+        for (int j = 0; j < 4; j++) s = fmaf(q[j], k[j], s);
+#pragma unroll
+        for (uint32_t d = 1; d < L; d *= 2) s += __shfl_xor(s, d, L);
+        s *= p.scale_log2;
+        const float now = s > m ? s : m, ref = now == -INFINITY ? 0.f : now, by = __builtin_amdgcn_exp2f(m - ref), f = __builtin_amdgcn_exp2f(s - ref);
+        m = now;
+        l = fmaf(l, by, f);
+#pragma unroll
+        for (int j = 0; j < 4; j++) o[j] = fmaf(f, v[j], o[j] * by);
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] *= inv;
+}
+
+// ---------------------------------------------------------------------------
 // The parts of every row brought to a common maximum and added in order: the prefix' parts, then the rest's.  HD / 4 lanes to a row and
 // every GROUPS-th part, whose sums meet in LDS: eight where the rows are few and may have been cut into very many parts, whose reads
 // would follow each other, else one.
@@ -1070,15 +1143,21 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
     __shared__ float2 part_ml[GROUPS][HPW];
     __shared__ __attribute__((aligned(16))) float part_o[GROUPS][HPW][HD];
     const uint32_t tid = threadIdx.x, c = tid % L, group = tid / L / HPW, per_tok = (a.nq + HPW - 1) / HPW;
-    for (uint64_t w = blockIdx.x; w < (uint64_t)a.n_tokens * per_tok; w += gridDim.x) {
+    const uint64_t all = (uint64_t)a.n_tokens * per_tok, each = (all + gridDim.x - 1) / gridDim.x, w1 = min(all, (blockIdx.x + 1) * each);
+    uint32_t r = 0xFFFFFFFFu, r_tok = 0xFFFFFFFFu;  // the request of token r_tok
+    for (uint64_t w = blockIdx.x * each; w < w1; w++) {  // (one after the other: a token's heads look for its request once)
         const uint32_t t = (uint32_t)(w / per_tok), hl = tid / L % HPW, h = (uint32_t)(w % per_tok) * HPW + hl;
-        __syncthreads();
-        if (tid == 0) found = 0xFFFFFFFFu;
-        __syncthreads();
-        for (uint32_t r = tid; r < a.n_requests; r += 256)
-            if (a.d_cu_tokens[r] <= (int)t && (int)t < a.d_cu_tokens[r + 1]) found = r;
-        __syncthreads();
-        const uint32_t r = found;
+        if constexpr (GROUPS > 1) __syncthreads();
+        if (t != r_tok) {
+            __syncthreads();
+            if (tid == 0) found = 0xFFFFFFFFu;
+            __syncthreads();
+            for (uint32_t i = tid; i < a.n_requests; i += 256)
+                if (a.d_cu_tokens[i] <= (int)t && (int)t < a.d_cu_tokens[i + 1]) found = i;
+            __syncthreads();
+            r = uniform(found);
+            r_tok = t;
+        }
         if (r == 0xFFFFFFFFu) continue;
         const uint32_t kvh = min(h, a.nq - 1) / p.G;
         // This row's parts of an entry: `n` of them, one in each share that its unit's blocks lie in, a tile apart.
@@ -1097,8 +1176,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
             tile0 = shared.tile;
         }
         const uint32_t at1 = parts(rest, n1);
-        // (a row with one part was written by the share that had it)
-        const uint32_t n = h >= a.nq || (!rest.parts && n1 <= 1) ? 0u : n0 + n1;
+        // (a row with one part was written by the share that had it, which left the sum of its outputs in the maximum's place)
+        const bool whole = !rest.parts && n1 <= 1;
+        const uint32_t n = h >= a.nq || whole ? 0u : n0 + n1;
+        const float2 left = whole && n1 == 1 && h < a.nq && group == 0 ? p.ml[at1] : make_float2(0.f, 0.f);
         // every lane reads one part's maximum and sum, then all read the parts' outputs together
         float m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
         for (uint32_t i0 = group * L; i0 < n; i0 += L * GROUPS) {
@@ -1160,12 +1241,22 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
                 }
             }
         }
-        if (n == 0 || group) continue;
-        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        if (group) continue;
+        float odd = left.x;
+        if (n) {
+            const float inv = l == 0.f ? 0.f : 1.0f / l;
 #pragma unroll
-        for (int i = 0; i < 4; i++) o[i] *= inv;
+            for (int i = 0; i < 4; i++) o[i] *= inv;
+            odd = (o[0] + o[1]) + (o[2] + o[3]);
+        } else {
+            l = left.y;
+        }
+        const unsigned long long row_lanes = __builtin_amdgcn_ballot_w64(odd - odd != 0.f && l - l == 0.f) >> (tid & 63u & ~(L - 1));
+        const bool again = (L == 64 ? row_lanes : row_lanes & ((1ull << (L % 64)) - 1)) != 0;
+        if (again) pa_row_again<HD>(p, r, t, h, c, o);
+        if (n == 0 && !again) continue;
         pa_store4(a.d_out, a.dtype, (size_t)t * a.out_stride + (size_t)h * HD + 4 * c, o);
-        if (c == 0 && a.d_lse) a.d_lse[(size_t)t * a.nq + h] = pa_lse(m, l);
+        if (n && c == 0 && a.d_lse) a.d_lse[(size_t)t * a.nq + h] = pa_lse(m, l);
     }
 }
 

@@ -363,3 +363,31 @@ def test_attention_heads_and_pages(backend, heads, dtype, kv, page):
     nq, nkv, hd = heads
     Attention([(150, [(40, 1), (5, 1), (77, 9)]), (0, [(260, 1)])], nq=nq, nkv=nkv, hd=hd, page=page, dtype=dtype, kv=kv, seed=page + hd, pad_rows=3,
               tail=2).run().expect().check()
+
+
+@pytest.mark.parametrize("dtype,kv", TYPES)
+@pytest.mark.parametrize("heads", [(8, 2, 128), (6, 2, 64), (3, 3, 256)], ids=str)
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_attention_values_that_only_later_rows_see(backend, heads, dtype, kv, what):
+    """A key's value that is no number, or infinite, reaches the rows that see the key and no others."""
+    nq, nkv, hd = heads
+    a = Attention([(0, [(50, 50), (90, 13), (3, 3)]), (20, [(9, 2), (9, 3), (30, 1)]), (70, [(40, 40), (33, 35)]), (0, [(1500, 5)])], nq=nq, nkv=nkv, hd=hd, page=16,
+                  dtype=dtype, kv=kv, seed=hd)
+    for r in range(len(a.lens)):
+        n = int(a.cu[r + 1] - a.cu[r])
+        for at in {int(a.lens[r]) - 1, int(a.lens[r]) - (n + 1) // 2}:
+            page, row = a.tables[r, at // 16], at % 16
+            if kv == "f16":
+                a.rows[1][:, page, row, at % hd] = what
+            elif kv == "fp8" and np.isnan(what):
+                a.rows[1][:, page, row, at % hd] = 0x7f
+            else:
+                a.scales[1][:, page, row] = what
+    a.make()
+    with np.errstate(invalid="ignore"):
+        a.run().expect().check()
+        out, got = a.want[0], pm.from_type(a.dout.get(), dtype)
+        odd = ~np.isfinite(out)
+        assert odd.any() and np.isfinite(out).any()
+        assert np.array_equal(np.isfinite(got), ~odd)
+        assert np.array_equal(got[odd], out[odd], equal_nan=True)
