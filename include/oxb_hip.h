@@ -239,7 +239,8 @@ int  oxb_hip_kv_dequantize_rows(int kv_dtype, const uint8_t* codes, const float*
  * pointer that the caller owns, also the workspace; the calls launch on the stream in use, allocate nothing, wait for nothing
  * and keep nothing, so they may be captured into a graph, which then reads whatever the buffers hold at each replay.  Lengths
  * and page numbers live on the GPU and cannot be refused by a call: what they may name is checked by the kernels, and no value
- * makes them leave their buffers.  The library runs on one device (oxb_hip_init): a pointer of another one is refused. */
+ * makes them leave their buffers.  The calls run on the library's device (oxb_hip_init), whatever device is the caller's current
+ * one; buffers are that device's (pointers are not looked at for it). */
 enum { OXB_DTYPE_F32 = 0, OXB_DTYPE_F16 = 1, OXB_DTYPE_BF16 = 2 };
 /* One layer's rows: k, v [nkv][n_pages][page_size][hd], fp16 numbers or one-byte codes (OXB_KV_DTYPE_*), 16-byte aligned; one-byte
  * rows with their scales [nkv][n_pages][page_size] (>= 0).  This is how a model keeps the rows of a layer in a paged cache.  A
@@ -306,6 +307,10 @@ int  oxb_hip_paged_rows_dev(const oxb_paged_rows* a);
  * shared; else cu_groups[0] = 0 and cu_groups[n_groups] = n_requests.
  * q, out: one type (f32: fp32-level accuracy, scores and probabilities as two fp16 terms; f16, bf16: probabilities are
  * rounded to fp16).  Strides in elements, multiples of 8; 16-byte aligned.  scale 0 stands for 1 / sqrt(hd).  n_requests 1 .. 4096.
+ * A value that is infinite or no number reaches the queries that see its key and no others; such queries are slow (a key at a
+ * time).  Scales of value rows keep this accuracy from 2^-40 on; smaller ones lose what lies below 2^-65.
+ * Queries times table_width are limited: n_tokens nq / 16 + (n_requests + n_groups) nkv tiles of rows, twice that with groups, times
+ * table_width page_size / 32 + 20 blocks of keys have to be below 2^31.
  * d_workspace: oxb_hip_paged_attention_workspace bytes (at the same counts, no GPU needed, pointers are not looked at), 256-byte
  * aligned, contents of no meaning before and after; calls that overlap in time need one each. */
 typedef struct {

@@ -400,10 +400,10 @@ __device__ __forceinline__ void pa_store4(void* out, uint32_t dtype, size_t at, 
         *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(out) + at) =
             make_uint2(pa_bits16(v[0], dtype) | pa_bits16(v[1], dtype) << 16, pa_bits16(v[2], dtype) | pa_bits16(v[3], dtype) << 16);
 }
-// The exponent of a value row's scale, -100 .. 100: a smaller one counts as 2^-100, so that no probability relative to it overflows; a
-// larger one, or none, as 2^100, so that the sum of the probabilities does not vanish beside it (fp16 probabilities that overflow
-// for it make outputs that are not finite, and the row is done again).
-__device__ __forceinline__ float pa_exponent(float scale) { return (float)((int)(min(max(__float_as_uint(scale) & 0x7FFFFFFFu, 27u << 23), 227u << 23) >> 23) - 127); }
+// The exponent of a value row's scale, -40 .. 70: a smaller one counts as 2^-40, so that no probability relative to it overflows, a
+// larger one, or none, as 2^70.  Sums of probabilities relative to both ends still meet in fp32 (2^40 times 2^-110).  fp16
+// probabilities that overflow for a scale above that make outputs that are not finite, and such a row is done again.
+__device__ __forceinline__ float pa_exponent(float scale) { return (float)((int)(min(max(__float_as_uint(scale) & 0x7FFFFFFFu, 87u << 23), 197u << 23) >> 23) - 127); }
 // Natural logarithm of the sum from its maximum in log2 units.
 __device__ __forceinline__ float pa_lse(float m, float l) { return l > 0.f ? (m + log2f(l)) * 0.693147180559945309417f : l == 0.f ? -INFINITY : NAN; }
 

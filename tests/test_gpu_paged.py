@@ -391,3 +391,305 @@ def test_attention_values_that_only_later_rows_see(backend, heads, dtype, kv, wh
         assert odd.any() and np.isfinite(out).any()
         assert np.array_equal(np.isfinite(got), ~odd)
         assert np.array_equal(got[odd], out[odd], equal_nan=True)
+
+
+SMALL = dict(nq=8, nkv=2, hd=64, page=16)
+MIXED = [(40, [(3, 1), (20, 5), (17, 1)]), (0, [(60, 41)])]
+
+
+@pytest.mark.parametrize("page", [-1, None, 1 << 30, -(1 << 31)])
+@pytest.mark.parametrize("dtype,kv", TYPES[::2])
+def test_attention_page_numbers_that_are_none(backend, page, dtype, kv):
+    """They stay inside the pool, and other requests' answers are right."""
+    a = Attention([(0, [(60, 1)]), (0, [(50, 1), (70, 30)]), (33, [(20, 2), (9, 1)])], **SMALL, dtype=dtype, kv=kv, seed=3)
+    n_pages = a.rows[0].shape[1]
+    a.expect()
+    a.tables[1:3, 1::2] = n_pages if page is None else page
+    a.make()
+    a.run()
+    bad = np.zeros(a.t, bool)
+    bad[a.cu[1]:a.cu[3]] = True
+    out, lse, mag, low = a.want
+    got, got_lse = a.dout.get(), a.dlse.get()
+    got[bad], got_lse[bad] = pm.to_type(out[bad], dtype), lse[bad]
+    a.dout.put(got)
+    a.dlse.put(got_lse)
+    a.check()
+
+
+@pytest.mark.parametrize("what", ["tokens", "groups"])
+def test_attention_sums_that_do_not_ascend_do_nothing(backend, what):
+    a = Attention(MIXED, **SMALL, dtype="float16", kv="f16")
+    if what == "tokens":
+        a.cu = np.array([0, 6, 1, 7, a.t])
+    else:
+        a.cu_g = [0, 5, 4]
+    a.make()
+    a.run()
+    assert np.all(a.dout.get() == 9.0) and np.all(a.dlse.get() == 9.0)
+
+
+@pytest.mark.parametrize("dtype,kv", TYPES)
+def test_attention_positions_and_lengths_at_their_ends(backend, dtype, kv):
+    a = Attention([(0, [(60, 4)]), (0, [(50, 3), (70, 30)]), (33, [(20, 2), (9, 1)])], **SMALL, dtype=dtype, kv=kv, seed=3)
+    a.pos = a.pos.astype(np.int64)
+    a.pos[[1, 5, 20]] = 2 ** 31 - 1, -(2 ** 31), 0
+    a.lens[1] = -5
+    a.make()
+    a.run().expect().check()
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.01, 1.0])
+@pytest.mark.parametrize("dtype,kv", TYPES)
+def test_attention_scales(backend, scale, dtype, kv):
+    a = Attention(MIXED, **SMALL, dtype=dtype, kv=kv, seed=4, scale=scale, spread=0.5)
+    a.run().expect()
+    a.size = np.abs(a.size)
+    a.check()
+
+
+@pytest.mark.parametrize("dtype,kv", TYPES)
+def test_attention_strided_rows(backend, dtype, kv):
+    """q as a slice of a product's rows, out as a slice of something wider: what lies beside them stays."""
+    a = Attention(MIXED, **SMALL, dtype=dtype, kv=kv, seed=5, pad_rows=2)
+    wide, own = a.nq * a.hd, a.nq * a.hd
+    q = np.full((a.t, wide + 256), np.nan)
+    q[:, 128:128 + own] = pm.from_type(a.q, dtype).reshape(a.t, -1)
+    base, out = DevArray(pm.to_type(q, dtype), dtype), DevArray(pm.to_type(np.full((a.t, wide + 72), 9.0), dtype), dtype)
+    a.call(base.view(128, (a.t, a.nq, a.hd), (wide + 256, a.hd, 1)), out.view(64, (a.t, a.nq, a.hd), (wide + 72, a.hd, 1)), lse=None, workspace=a.ws)
+    got = out.get()
+    beside = pm.from_type(got, dtype)
+    assert np.all(beside[:, :64] == 9.0) and np.all(beside[:, 64 + own:] == 9.0)
+    assert np.all(a.dlse.get() == 9.0)
+    a.run()
+    whole = a.dout.get()
+    assert np.array_equal(whole.reshape(a.t, -1), got[:, 64:64 + own])       # the same bits, with lse and without
+    a.expect().check()
+
+
+@pytest.mark.parametrize("kv", ["i8", "fp8"])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("how", ["wide", "ends", "huge"])
+def test_attention_value_scales_far_apart(backend, kv, dtype, how):
+    a = Attention([(100, [(30, 1), (9, 3)]), (0, [(260, 60), (40, 40)])], **SMALL, dtype=dtype, kv=kv, seed=6)
+    s = a.scales[1]
+    keys = a.rng.random(s.shape)
+    if how == "wide":
+        s[:] = np.where(np.isnan(s), s, 2.0 ** (40 * keys - 20)).astype(np.float32)
+    elif how == "ends":
+        s[:] = np.where(np.isnan(s), s, np.where(keys < 0.1, 2e-38, np.where(keys > 0.97, 1e30, s)))
+    else:
+        for r in range(4):       # one key of each request, which all its rows see
+            s[:, a.tables[r, 0], 7] = 1e35
+    a.make()
+    a.run().expect().check()
+
+
+@pytest.mark.parametrize("how", ["alone", "groups", "most"])
+@pytest.mark.parametrize("dtype,kv", [("float16", "f16"), ("float32", "i8")])
+def test_attention_of_many_requests(backend, how, dtype, kv):
+    rng = np.random.default_rng(8)
+    if how == "alone":
+        groups = [(0, [(int(rng.integers(1, 60)), 1)]) for _ in range(700)]
+    else:
+        groups, left = [], 4096 if how == "most" else 400
+        while left:
+            n = min(left, int(rng.integers(1, 8)))
+            groups.append((int(rng.integers(0, 40)), [(int(rng.integers(4, 30)), int(rng.choice([0, 1, 1, 1, 1, 3]))) for _ in range(n)]))
+            left -= n
+    a = Attention(groups, nq=4, nkv=1, hd=32, page=16, dtype=dtype, kv=kv, seed=9, share=how != "alone", poison=False)
+    a.run().expect().check()
+
+
+def test_rows_and_attention_far_into_a_large_pool(backend):
+    """Rows past 2^31 elements and 2^32 bytes of the pool."""
+    a = Attention([(140, [(3, 1), (200, 1)]), (0, [(300, 70)])], nq=8, nkv=2, hd=128, page=128, dtype="float16", kv="f16", poison=False)
+    n_pages, page, hd = 100000, 128, 128
+    small = a.rows[0].shape[1]
+
+    def big():
+        d = object.__new__(DevArray)
+        d.host, d.dtype, d.first, d.shape = np.empty(1, np.float16), "x.float16", 0, (2, n_pages, page, hd)
+        d._stride, d.buf = (n_pages * page * hd, page * hd, hd, 1), DeviceBuffer(2 * n_pages * page * hd * 2)
+        return d
+
+    far = {p: n_pages - 1 - 37 * p for p in range(small)}
+    pools = [big(), big()]
+    try:
+        hip = DeviceBuffer.hip()
+        for d, rows in zip(pools, a.rows):
+            for h in range(2):
+                for p in range(small):
+                    block = np.ascontiguousarray(rows[h, p])
+                    assert hip.hipMemcpy(d.buf.ptr + (h * n_pages + far[p]) * page * hd * 2, block.ctypes.data, block.nbytes, 1) == 0
+        tables = np.vectorize(lambda p: far.get(p, -1))(a.tables).astype(np.int32)
+        pool = paged.PagePool(*pools)
+        a.dev["tables"] = _i32(tables)
+        call = paged.PagedAttention(pool, nq=8, **a.dev)
+        call(a.dq, a.dout, lse=a.dlse, workspace=a.ws)
+        a.expect().check()
+        slots = [far[0] * page + 5, far[1] * page + 127]
+        x = a.rng.standard_normal((2, 12 * hd)).astype(np.float16)
+        paged.RowStore(pool, nq=8, slots=_i32(slots))(DevArray(x))
+        for i, s in enumerate(slots):
+            for h in range(2):
+                for d, at in ((pools[0], 8 + h), (pools[1], 10 + h)):
+                    row = np.empty(hd, np.float16)
+                    assert hip.hipDeviceSynchronize() == 0
+                    assert hip.hipMemcpy(row.ctypes.data, d.buf.ptr + (h * n_pages * page + s) * hd * 2, hd * 2, 2) == 0
+                    assert np.array_equal(row, x[i, at * hd:(at + 1) * hd])
+    finally:
+        for d in pools:
+            d.buf.free()
+
+
+def _graphs():
+    hip = DeviceBuffer.hip()
+    for f, args in (("hipStreamCreate", [C.POINTER(C.c_void_p)]), ("hipStreamDestroy", [C.c_void_p]), ("hipStreamBeginCapture", [C.c_void_p, C.c_int]),
+                    ("hipStreamEndCapture", [C.c_void_p, C.POINTER(C.c_void_p)]), ("hipStreamSynchronize", [C.c_void_p]),
+                    ("hipGraphInstantiate", [C.POINTER(C.c_void_p), C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
+                    ("hipGraphLaunch", [C.c_void_p, C.c_void_p]), ("hipGraphExecDestroy", [C.c_void_p]), ("hipGraphDestroy", [C.c_void_p])):
+        getattr(hip, f).argtypes = args
+    return hip
+
+
+def test_attention_on_two_streams_at_once(backend):
+    hip = _graphs()
+    calls = [Attention([(400, [(30, 1)] * 9)], nq=8, nkv=2, hd=128, page=16, dtype="float16", kv="f16", seed=1),
+             Attention([(70, [(90, 60), (20, 1)])], nq=8, nkv=2, hd=128, page=16, dtype="float32", kv="i8", seed=2)]
+    streams = [C.c_void_p(0), C.c_void_p(0)]
+    for s in streams:
+        assert hip.hipStreamCreate(C.byref(s)) == 0
+    try:
+        for _ in range(20):
+            for a, s in zip(calls, streams):
+                backend.set_stream(s.value)
+                a.run()
+        for s in streams:
+            assert hip.hipStreamSynchronize(s) == 0
+    finally:
+        backend.set_stream(0)
+        for s in streams:
+            assert hip.hipStreamDestroy(s) == 0
+    for a in calls:
+        a.expect().check()
+
+
+class Step(Attention):
+    """A server's step as it is used: pages, rows, attention, on buffers that stay."""
+
+    def __init__(self, groups, *, nq, nkv, hd, page, dtype, kv, n_rows, seed=0):
+        rng = self.rng = np.random.default_rng(seed)
+        self.nq, self.nkv, self.hd, self.page, self.dtype, self.kv, self.t, self.share = nq, nkv, hd, page, dtype, kv, n_rows, True
+        self.scale = hd ** -0.5
+        b, width, n_pages, most = sum(n for _, n in groups), 24, 300, 400
+        self.prefix, self.cu_g = [p for p, _ in groups], np.concatenate([[0], np.cumsum([n for _, n in groups])])
+        order, at = rng.permutation(n_pages).astype(np.int32), 0
+        self.tables = np.full((b, width), -1, np.int32)
+        for g, (p, _) in enumerate(groups):
+            assert p % page == 0
+            self.tables[self.cu_g[g]:self.cu_g[g + 1], :p // page] = order[at:at + p // page]
+            at += p // page
+        self.free, self.n_free = np.full(n_pages, -7, np.int32), n_pages - at
+        self.free[:self.n_free] = order[at:]
+        self.lens = np.repeat(self.prefix, [n for _, n in groups])
+        self.rows, self.scales = make_pool(rng, kv, nkv, n_pages, page, hd)
+        self.pool, self.dpool = dev_pool(self.rows, self.scales, kv)
+        angle = rng.random((most, hd // 2)) * 6
+        self.cos, self.sin = np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+        self.w = (0.5 + rng.random((2, hd))).astype(np.float32)
+        self.d = d = dict(past=_i32(self.lens), keep=_i32(self.lens), add=_i32(np.zeros(b)), tables=_i32(self.tables), free_pages=_i32(self.free), n_free=_i32([self.n_free]),
+                          cu_tokens=_i32(np.zeros(b + 1)), cu_pages=_i32(np.zeros(b + 1)), slots=_i32(np.zeros(n_rows)), positions=_i32(np.zeros(n_rows)), status=_i32([9, 9]))
+        self.assign = paged.PageAssign(page_size=page, lens=d["past"], **d)
+        self.store = paged.RowStore(self.pool, nq=nq, slots=d["slots"], positions=d["positions"], q_norm=DevArray(self.w[0]), k_norm=DevArray(self.w[1]), cos=DevArray(self.cos),
+                                    sin=DevArray(self.sin), eps=1e-6)
+        self.call = paged.PagedAttention(self.pool, nq=nq, tables=d["tables"], cu_tokens=d["cu_tokens"], positions=d["positions"], lens=d["past"], cu_groups=_i32(self.cu_g),
+                                         prefix_lens=_i32(self.prefix))
+        self.ws = DevArray(np.full(self.call.workspace_bytes // 4, np.nan, np.float32))
+        self.dqkv = DevArray(np.zeros((n_rows, (nq + 2 * nkv) * hd), np.float32))
+        self.dq, self.dout = (DevArray(pm.to_type(np.full((n_rows, nq, hd), 9.0), dtype), dtype) for _ in range(2))
+        self.dlse = DevArray(np.full((n_rows, nq), 9.0, np.float32))
+
+    def launch(self):
+        self.assign()
+        self.store(self.dqkv, self.dq)
+        self.call(self.dq, self.dout, lse=self.dlse, workspace=self.ws)
+
+    def step(self, keep, add, run):
+        """New lengths and rows, the step by run(), and everything against the plain forms."""
+        self.d["keep"].put(keep)
+        self.d["add"].put(add)
+        x = self.rng.standard_normal((self.t, self.nq + 2 * self.nkv, self.hd)).astype(np.float32)
+        self.dqkv.put(x.reshape(self.t, -1))
+        self.dout.put(pm.to_type(np.full(self.dout.shape, 9.0), self.dtype))
+        self.dlse.put(np.full(self.dlse.shape, 9.0))
+        run()
+        w = pm.assign(self.lens, keep, add, self.tables, self.free, self.n_free, self.page, self.t)
+        self.tables, self.free, self.n_free, self.lens, self.cu, self.pos = (w[n] for n in ("tables", "free", "n_free", "lens", "cu_tokens", "positions"))
+        for n in ("tables", "cu_tokens", "positions", "slots", "status"):
+            assert np.array_equal(self.d[n].get(), w[n]), n
+        assert np.array_equal(self.d["past"].get(), w["lens"]) and self.d["n_free"].get()[0] == w["n_free"]
+        n = int(self.cu[-1])
+        at = self.pos[:n]
+        turned = [pm.turned(x[:n, lo:hi], wt, self.cos[at], self.sin[at], 1e-6)
+                  for lo, hi, wt in ((0, self.nq, self.w[0]), (self.nq, self.nq + self.nkv, self.w[1]))]
+        self.q = self.dq.get()
+        err = np.abs(pm.from_type(self.q, self.dtype)[:n] - turned[0])
+        assert np.all(err <= HALF_STEP[self.dtype] * np.abs(turned[0]) + (64 + self.hd) * U * np.abs(turned[0]).max(-1, keepdims=True) + 2.0 ** -25)
+        k = [d.get() for d in self.dpool if d is not None]
+        self.rows, self.scales = k[:2], k[2:] or [None, None]
+        stored = pm.pool_values(self.rows[0], self.scales[0], self.kv)[:, w["slots"][:n] // self.page, w["slots"][:n] % self.page].transpose(1, 0, 2)
+        top = np.abs(turned[1]).max(-1, keepdims=True)
+        step = {"f16": 2.0 ** -11 * np.abs(turned[1]) + 2.0 ** -25, "i8": top / 127 / 2 * 1.001, "fp8": 2.0 ** -4 * np.abs(turned[1]) + top / 448 * 2.0 ** -10}[self.kv]
+        assert np.all(np.abs(stored - turned[1]) <= step + 2 * (64 + self.hd) * U * top)
+        self.expect().check()
+
+
+PLAN = [("add", [37, 5, 12, 0, 50, 3]), ("one", None), ("one", None), ("draft", 4), ("reject", 1), ("end", [2, 4]), ("add", [1, 1, 30, 1, 21, 1]), ("one", None)]
+
+
+@pytest.mark.parametrize("dtype,kv", TYPES)
+@pytest.mark.parametrize("graph", [False, True])
+def test_steps_of_a_server(backend, dtype, kv, graph):
+    """Chunks, single tokens, drafts, requests that end and others in their place: every step the same three calls, eagerly or as
+    one captured graph that reads the lengths of its replay."""
+    hip = _graphs()
+    s = Step([(32, 2), (0, 1), (64, 3)], nq=8, nkv=2, hd=64, page=16, dtype=dtype, kv=kv, n_rows=130, seed=11)
+    other = Attention(MIXED, **SMALL, dtype=dtype, kv=kv, seed=5)
+    prefix = np.repeat(s.prefix, np.diff(s.cu_g))
+    stream, graph_, gexec = C.c_void_p(0), C.c_void_p(0), C.c_void_p(0)
+    run = s.launch
+    try:
+        if graph:
+            assert hip.hipStreamCreate(C.byref(stream)) == 0
+            backend.set_stream(stream.value)
+            assert hip.hipStreamBeginCapture(stream, 0) == 0
+            s.launch()
+            assert hip.hipStreamEndCapture(stream, C.byref(graph_)) == 0
+            assert hip.hipGraphInstantiate(C.byref(gexec), graph_, None, None, 0) == 0
+
+            def run():
+                assert hip.hipGraphLaunch(gexec, stream) == 0
+                assert hip.hipStreamSynchronize(stream) == 0
+        for what, arg in PLAN:
+            keep, add = s.lens.copy(), np.ones(6, np.int32)
+            if what == "add":
+                add = np.array(arg)
+            elif what == "draft":
+                add[:] = arg
+            elif what == "reject":
+                keep -= 3
+                add[:] = arg
+            elif what == "end":
+                keep[arg], add[arg] = prefix[arg], 0
+            s.step(keep, add, run)
+            other.run()
+        other.expect().check()
+    finally:
+        backend.set_stream(0)
+        if gexec:
+            hip.hipGraphExecDestroy(gexec)
+        if graph_:
+            hip.hipGraphDestroy(graph_)
+        if stream:
+            hip.hipStreamDestroy(stream)
