@@ -96,7 +96,8 @@ int oxb_hip_paged_rows_dev(const oxb_paged_rows* a) {
     if (int rc = check_pool(a->pool)) return rc;
     if (a->n_rows == 0 || a->n_rows > (1u << 30)) return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: %u rows (1 .. 2^30)", a->n_rows);
     const uint64_t wide = ((uint64_t)a->nq + 2 * a->pool.nkv) * a->pool.hd;
-    if (a->nq > 16384 || (uint64_t)a->n_rows * wide / 2048 >= 0x7FFFFFFFu) return bad("rows too many and too wide for one launch");
+    if (a->nq > 16384 || (uint64_t)a->n_rows * wide / 8 > 0xFFFFFF00u)  // (a thread to eight values; a launch counts its threads in 32 bits)
+        return bad("rows too many and too wide for one launch");
     if (a->qkv_dtype > OXB_DTYPE_BF16 || (a->d_q_out && a->q_dtype > OXB_DTYPE_BF16)) return bad("unknown type of rows");
     if (!a->d_qkv || !a->d_slots || !aligned(a->d_qkv, 16) || !aligned(a->d_q_out, 16)) return bad("null or unaligned rows, or no slots");
     if (a->qkv_stride < wide || a->qkv_stride % 8) return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: row stride %u (a multiple of 8, at least %llu)", a->qkv_stride, (unsigned long long)wide);

@@ -176,3 +176,9 @@ def test_plain_attention_in_two_parts_is_one_softmax():
         for h in range(2):
             e = np.exp(kk @ q[t, h] * 0.3)
             assert np.allclose(out[t, h], e @ vv / e.sum()) and np.isclose(lse[t, h], np.log(e.sum()))
+
+
+@pytest.mark.parametrize("n_rows", [(1 << 26) - 3, 1 << 26, 1 << 27, 1 << 30])
+def test_rows_of_more_threads_than_a_launch_has(n_rows):
+    assert rows(n_rows=n_rows) == INVALID
+    assert "too many" in _lib.last_error()
