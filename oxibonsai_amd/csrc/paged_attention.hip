@@ -16,6 +16,10 @@
 // Workgroups go to the eight XCDs in turn, shares go to them in runs, so that the tiles of a kv head, which walk the same keys, are near
 // each other.  The first workgroup of a CU takes from the first half, where the prefixes are, which are bound by the matrix
 // cores, the second one from the second half, where the rests are, which are bound by memory.
+//
+// Calls, 32 q heads on 8 kv heads of 128: 62 requests of 700 keys behind 4100 shared ones, fp16 rows, 40.5 us (107 MB, 22.7 us
+// at a copy's rate; 33 in the first launch = 3.2 TB/s), 256 of 900 behind 16 000 162 us (542 MB), 14 chunks of 300 behind 3500
+// 165 us (89 GFLOP, 0.6 PFLOP/s in the first launch), 90 requests of 400 behind 2000, INT8 rows, f32, 40.3 us.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -29,13 +33,13 @@ typedef uint32_t v4w __attribute__((ext_vector_type(4)));
 typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 
 #define PA_SHARES 512u     // workgroups: two to a CU
-#define PA_FEW 32u         // rows up to which an entry's tiles have 16 rows and a wave to themselves
+#define PA_FEW 32u         // rows up to which an entry's tiles have 16 rows and a wave to themselves (16: the same; 48: 36 rows over 60 000 keys 76 us instead of 52)
 #define PA_TILE_FEW_LOG 4u
 #define PA_KEYS_FEW_LOG 5u // keys that such a wave takes at a time: 32
 #define PA_RUNS 256u       // runs of entries, one to a thread
 #define PA_STAGED 240u     // requests up to which a workgroup copies the lengths to LDS first
-#define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk
-#define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes
+#define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk (48, 1600: within 1 %)
+#define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes (100: 9 questions about 60 000 keys 59.5 us instead of 54)
 #define PA_LOG2E 1.44269504088896340736f
 
 // Rows of a tile of many rows, and keys of a block of theirs, by what the registers and two workgroups' LDS hold.  Entries of up to 64
@@ -676,9 +680,9 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
 // one-byte rows wait in registers and are widened on their way.  The rows' 16-byte pieces are permuted by an XOR with the
 // row number, so that neither the reads of K (16 rows, one piece) nor the transposing reads of V meet in a bank.
 //
-// The same products and softmax as above; V's operand comes from the transposing reads.  Bound by the matrix cores, the LDS
-// reads (two tiles share an operand) and the VALU's softmax about equally: 512 cycles each per 32 keys of head_dim 128 and
-// wave.
+// The same products and softmax as above; V's operand comes from the transposing reads.  Bound by issue: matrix instructions (0.27
+// of the SIMDs' time in 14 chunks of 300 queries behind 3500 keys), LDS reads, of which two tiles share each, and the VALU's softmax;
+// 0.30 of the waves' time waits for its turn to issue.
 // ---------------------------------------------------------------------------
 // K and V of two blocks: arrays of their own, so that the compiler sees that a read of one need not wait for what is on its way
 // to another.
@@ -1133,7 +1137,7 @@ __device__ __forceinline__ void pa_row_again(const PaParams& p, uint32_t r, uint
 // ---------------------------------------------------------------------------
 // The parts of every row brought to a common maximum and added in order: the prefix' parts, then the rest's.  HD / 4 lanes to a row and
 // every GROUPS-th part, whose sums meet in LDS: eight where the rows are few and may have been cut into very many parts, whose reads
-// would follow each other, else one.
+// would follow each other, else one.  Latency bound: 5.5 us for 80 rows, 7 for 1984, 24 for 134 000 that were whole already.
 // ---------------------------------------------------------------------------
 template <int HD, int GROUPS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {

@@ -16,7 +16,8 @@
 // has - held and add over the requests give every freed page its place on the stack of free pages, every new page the entry it
 // comes from and every token its row.  One workgroup works the sums out (the numbers of a step fit its LDS: 4096 requests are
 // three arrays of 16 KB) and moves the freed pages; the tokens' slots follow in the same launch while they are few, else in a
-// second one over the whole chip.  Latency bound: a trip to memory for the lengths, one for a page given up, one for a table entry.
+// second one over the whole chip.  Latency bound: a trip to memory for the lengths, one for a page given up, one for a table entry;
+// 4.6 us for 24 single tokens, 5.6 and 6 to 8 (two launches) for the 280 000 rows of 500 prompts.
 // ---------------------------------------------------------------------------
 #define PAGES_THREADS 1024
 #define PAGES_ROWS_PER_WG 1024     // of the second launch
@@ -209,7 +210,8 @@ hipError_t oxb_launch_paged_assign(const oxb_page_assign& a, hipStream_t st) {
 //
 // HD / 8 lanes share a head: a lane has four dimensions of each half, so both members of a rotation pair are its own and only the
 // sum of squares (and a one-byte row's largest) crosses lanes.  Everything is read and written once, nothing waits for anything
-// but the row's position and slot: bound by memory.
+// but the row's position and slot: bound by memory, 48 us for 8192 tokens of 32 + 2 x 8 heads of 128, bf16 to fp16 (195 MB, 4.1 TB/s),
+// 13.2 us for 2999 to INT8 rows (64 MB); a launch's latency for few rows (17 tokens 3.2 us).
 // ---------------------------------------------------------------------------
 template <int DT>
 __device__ __forceinline__ void rows_load4(const void* p, size_t at, float v[4]) {
