@@ -1075,8 +1075,8 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 // ---------------------------------------------------------------------------
 // A row over again, key by key and only the keys that it sees, by HD / 4 lanes.  The products of a block that only some of its rows see
 // multiply the values of a key that a row does not see by 0, which is no number where that value, or its row's scale, is infinite or
-// none itself: such rows, a finite sum of probabilities beside an output that is not finite, come here.  Slow (a key at a time, about
-// 1 us each) and rare; with infinities that the row does see the answer is the same as before.
+// none itself: such rows, a finite sum of probabilities beside an output that is not finite, come here.  Slow (a key at a time)
+// and rare; with infinities that the row does see the answer is the same as before.
 // ---------------------------------------------------------------------------
 template <int HD>
 __device__ __forceinline__ void pa_row_again(const PaParams& p, uint32_t r, uint32_t t, uint32_t h, uint32_t c, float o[4]) {

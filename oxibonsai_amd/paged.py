@@ -11,7 +11,7 @@ step and layer (``RowStore``, ``PagedAttention``):
 The reference keeps its tables on the host and its rows one token at a time (``PagedKvCache``,
 crates/oxibonsai-model/src/paged_kv_cache.rs:294-470).  Buffers are anything with ``data_ptr()``, ``shape``, ``stride()``,
 ``dtype`` and ``device`` (torch tensors); they stay the caller's and have to live as long as the object.  Calls run on
-the library's stream (``NativeHipBackend.set_stream``) and wait for nothing; they may be captured into a graph.  What the
+the library's stream (``NativeHipBackend.set_stream``) and wait for nothing; they may be captured into a graph.  An object takes calls of one thread at a time.  What the
 fields mean stands at the C structs of the same names, include/oxb_hip.h."""
 from __future__ import annotations
 
@@ -180,6 +180,8 @@ class PagedAttention(_Bound):
         c.d_out, kind, c.out_stride = _rows(out, "out", self.n, self._wide, dev)
         if kind != c.dtype:
             raise _bad(f"q is {_kind(q)}, out {_kind(out)}")
+        if c.d_q == c.d_out:
+            raise _bad("out is q, which is still read while rows of out are written")
         c.d_lse = _flat(lse, "lse", "float32", (self.n, self.nq), dev)
         if not workspace.is_contiguous():
             raise _bad("the workspace is not contiguous")

@@ -693,3 +693,26 @@ def test_steps_of_a_server(backend, dtype, kv, graph):
             hip.hipGraphDestroy(graph_)
         if stream:
             hip.hipStreamDestroy(stream)
+
+
+@pytest.mark.parametrize("kind", ["float32", "float16", "bfloat16"])
+def test_rows_in_place(backend, kind):
+    """q back into the product's rows: the same bits as into a buffer of its own, k and v beside it as they were."""
+    rng = np.random.default_rng(2)
+    n, nq, nkv, hd = 9, 6, 2, 64
+    wide = (nq + 2 * nkv) * hd
+    x = pm.to_type(rng.standard_normal((n, wide)), kind)
+    angle = rng.random((20, hd // 2)) * 6
+    kw = dict(nq=nq, slots=_i32(np.arange(n) + 3), positions=_i32(np.arange(n) * 2), q_norm=DevArray(np.ones(hd, np.float32) * 1.5), k_norm=DevArray(np.ones(hd, np.float32)),
+              cos=DevArray(np.cos(angle).astype(np.float32)), sin=DevArray(np.sin(angle).astype(np.float32)))
+    rows, scales = make_pool(rng, "f16", nkv, 2, 16, hd)
+    got = []
+    for own in (True, False):
+        pool, d = dev_pool(rows, scales, "f16")
+        qkv, q = DevArray(x, kind), DevArray(pm.to_type(np.zeros((n, nq, hd)), kind), kind)
+        paged.RowStore(pool, **kw)(qkv, q if own else qkv.view(0, (n, nq, hd), (wide, hd, 1)))
+        after = qkv.get()
+        assert np.array_equal(after[:, nq * hd:], x[:, nq * hd:])
+        got.append((q.get().reshape(n, -1) if own else after[:, :nq * hd], d[0].get(), d[1].get()))
+    for a, b in zip(*got):
+        assert np.array_equal(a, b)

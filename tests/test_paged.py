@@ -182,3 +182,11 @@ def test_plain_attention_in_two_parts_is_one_softmax():
 def test_rows_of_more_threads_than_a_launch_has(n_rows):
     assert rows(n_rows=n_rows) == INVALID
     assert "too many" in _lib.last_error()
+
+
+def test_attention_into_its_own_queries_is_refused():
+    k = Host((2, 10, 16, 64), "float16")
+    a = paged.PagedAttention(paged.PagePool(k, k), nq=4, tables=ints(3, 4), cu_tokens=ints(4), positions=ints(5), lens=ints(3))
+    q = Host((5, 4, 64), "float16")
+    with pytest.raises(GpuError, match="out is q"):
+        a(q, q, workspace=Host((a.workspace_bytes,), "uint8"))
