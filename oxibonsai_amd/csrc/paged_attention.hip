@@ -1137,7 +1137,8 @@ __device__ __forceinline__ void pa_row_again(const PaParams& p, uint32_t r, uint
 // ---------------------------------------------------------------------------
 // The parts of every row brought to a common maximum and added in order: the prefix' parts, then the rest's.  HD / 4 lanes to a row and
 // every GROUPS-th part, whose sums meet in LDS: eight where the rows are few and may have been cut into very many parts, whose reads
-// would follow each other, else one.  Latency bound: 5.5 us for 80 rows, 7 for 1984, 24 for 134 000 that were whole already.
+// would follow each other, else one.  Latency bound: 5.5 us for 80 rows, 7 for 1984, 24 for 134 000 of 14 chunks, most
+// of whose tokens have rows in two shares (a look at all of a token's rows first: 27).
 // ---------------------------------------------------------------------------
 template <int HD, int GROUPS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
