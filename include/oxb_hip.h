@@ -49,8 +49,12 @@ int  oxb_hip_device_count(void);
 int  oxb_hip_device_info(char* name, size_t name_cap, size_t* free_bytes, size_t* total_bytes);
 /* GpuBackendTrait::synchronize (KG/mod.rs:403) */
 int  oxb_hip_synchronize(void);
-/* Run on the caller's HIP stream (hipStream_t passed as void*); NULL restores the library's own stream.
+/* Run on the caller's HIP stream (hipStream_t passed as void*); NULL restores the library's own stream, which waits for no
+ * other and no other waits for it.  HIP's null stream, where torch's default stream runs, has the handle 0: it is named
+ * OXB_HIP_NULL_STREAM here.  It belongs to the caller's current device, which has to be the library's for calls on it (the
+ * oxb_hip_paged_* calls see to that themselves).  The stream in use is the process's, not the thread's.
  * The decode step's graph is recorded on the library's own stream and replayed on the stream in use. */
+#define OXB_HIP_NULL_STREAM ((void*)1)
 int  oxb_hip_set_stream(void* hip_stream);
 const char* oxb_hip_last_error(void);
 

@@ -18,6 +18,8 @@ u32p = C.POINTER(C.c_uint32)
 u64p = C.POINTER(C.c_uint64)
 szp = C.POINTER(C.c_size_t)
 
+NULL_STREAM = 1  # OXB_HIP_NULL_STREAM
+
 _SIGNATURES = {
     "oxb_hip_init": ([C.c_int], C.c_int),
     "oxb_hip_shutdown": ([], None),

@@ -92,9 +92,10 @@ class NativeHipBackend:
     def synchronize(self, device_id: int = 0) -> None:
         _check(self._lib.oxb_hip_synchronize())
 
-    def set_stream(self, hip_stream: int = 0) -> None:
-        """Calls run on the caller's HIP stream from here on (``torch.cuda.Stream.cuda_stream``); 0 restores the library's own."""
-        _check(self._lib.oxb_hip_set_stream(hip_stream or None))
+    def set_stream(self, hip_stream: int | None = None) -> None:
+        """Calls run on the caller's HIP stream from here on (``torch.cuda.current_stream().cuda_stream``; 0 is the null stream, where
+        torch's default stream runs); None restores the library's own, which is ordered with no other."""
+        _check(self._lib.oxb_hip_set_stream(_lib.NULL_STREAM if hip_stream == 0 else hip_stream))
 
     def memory_info(self, device_id: int = 0) -> tuple[int, int]:
         """(free, total) bytes."""

@@ -476,7 +476,7 @@ int oxb_hip_set_stream(void* hip_stream) {
     std::lock_guard<std::recursive_mutex> lk(g_mu);
     int rc = ensure_init();
     if (rc) return rc;
-    g_rt.stream = hip_stream ? (hipStream_t)hip_stream : g_rt.own_stream;
+    g_rt.stream = !hip_stream ? g_rt.own_stream : hip_stream == OXB_HIP_NULL_STREAM ? nullptr : (hipStream_t)hip_stream;
     return OXB_HIP_OK;
     OXB_API_END
 }

@@ -194,6 +194,9 @@ pub struct OxbPagedAttention {
     pub pool: OxbPagePool,
 }
 
+/// What `oxb_hip_set_stream` takes for HIP's null stream, whose own handle is 0 (null restores the library's stream).
+pub const OXB_HIP_NULL_STREAM: *mut c_void = 1 as *mut c_void;
+
 extern "C" {
     // lifecycle
     pub fn oxb_hip_init(device_ordinal: c_int) -> c_int;

@@ -28,6 +28,14 @@ def backend():
     return ox.NativeHipBackend(0)
 
 
+@pytest.fixture(autouse=True)
+def own_stream(request):
+    """A test that has set a stream leaves the library's own to the next one."""
+    yield
+    if "backend" in request.fixturenames:
+        request.getfixturevalue("backend").set_stream(None)
+
+
 def pytest_collection_modifyitems(config, items):
     if _gpu_present():
         return

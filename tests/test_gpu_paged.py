@@ -10,6 +10,9 @@ Tolerances, from the arithmetic (u = 2^-24 of fp32, half a step of each rounding
    2^-25 whatever its size: of p s (s the row scale of v) relative to the row's largest, times |v| / s, so
    2^-25 max(p s) sum(|v| / s) / sum p"""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -716,3 +719,12 @@ def test_rows_in_place(backend, kind):
         got.append((q.get().reshape(n, -1) if own else after[:, :nq * hd], d[0].get(), d[1].get()))
     for a, b in zip(*got):
         assert np.array_equal(a, b)
+
+
+def test_calls_between_torch_operations(backend):
+    """The three calls on torch's default stream and on another of its streams, without a wait between them and torch's work."""
+    here = os.path.dirname(os.path.abspath(__file__))
+    env = dict(os.environ, PYTHONPATH=os.path.dirname(here))
+    r = subprocess.run([sys.executable, os.path.join(here, "paged_torch.py")], env=env, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert r.stdout.split("\n")[:2] == ["the default stream ok", "a side stream ok"]

@@ -4,12 +4,13 @@ import ctypes as C
 import os
 import shutil
 import subprocess
+from types import SimpleNamespace
 
 import numpy as np
 import pytest
 
 import paged_model as pm
-from oxibonsai_amd import GpuError, _lib, paged
+from oxibonsai_amd import GpuError, NativeHipBackend, _lib, paged
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 INVALID, NOT_AVAILABLE = 5, 1
@@ -190,3 +191,15 @@ def test_attention_into_its_own_queries_is_refused():
     q = Host((5, 4, 64), "float16")
     with pytest.raises(GpuError, match="out is q"):
         a(q, q, workspace=Host((a.workspace_bytes,), "uint8"))
+
+
+def test_the_null_stream_has_a_name_of_its_own():
+    seen = []
+    be = object.__new__(NativeHipBackend)
+    be._lib = SimpleNamespace(oxb_hip_set_stream=lambda handle: seen.append(handle) or 0)
+    for handle in (None, 0, 0x7f00):
+        be.set_stream(handle)
+    be.set_stream()
+    assert seen == [None, 1, 0x7f00, None]      # null restores the library's stream, 1 is OXB_HIP_NULL_STREAM
+    header = open(os.path.join(ROOT, "include", "oxb_hip.h")).read()
+    assert f"#define OXB_HIP_NULL_STREAM ((void*){_lib.NULL_STREAM})" in header
