@@ -203,7 +203,7 @@ def prepare(case, seed):
 # ---- the package's kernels: descriptors that a program makes once for its buffers ---------------------------------------
 def _bind(s):
     from oxibonsai_amd import NativeHipBackend, paged
-    NativeHipBackend(0)
+    NativeHipBackend(0).set_stream(torch.cuda.current_stream().cuda_stream)
     c = s["c"]
     if c["op"] == "pages":
         s["call"] = paged.PageAssign(past=s["past"], keep=s["keep"], add=s["add"], tables=s["tables"], free_pages=s["free"], n_free=s["n_free"],
