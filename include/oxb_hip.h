@@ -312,7 +312,7 @@ int  oxb_hip_paged_rows_dev(const oxb_paged_rows* a);
  * q, out: one type (f32: fp32-level accuracy, scores and probabilities as two fp16 terms; f16, bf16: probabilities are
  * rounded to fp16).  Strides in elements, multiples of 8; 16-byte aligned; no row of out overlaps one of q.  scale 0 stands for 1 / sqrt(hd).  n_requests 1 .. 4096.
  * A value that is infinite or no number reaches the queries that see its key and no others; such queries are slow (a key at a
- * time).  Scales of value rows keep this accuracy from 2^-40 on; smaller ones lose what lies below 2^-65.
+ * time).  Scales of value rows keep this accuracy from 2^-40 on; smaller ones lose what lies below 2^-79.
  * Queries times table_width are limited: n_tokens nq / 16 + (n_requests + n_groups) nkv tiles of rows, twice that with groups, times
  * table_width page_size / 32 + 20 blocks of keys have to be below 2^31.
  * d_workspace: oxb_hip_paged_attention_workspace bytes (at the same counts, no GPU needed, pointers are not looked at), 256-byte

@@ -41,6 +41,11 @@ typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 #define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk (48, 1600: within 1 %)
 #define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes (100: 9 questions about 60 000 keys 59.5 us instead of 54)
 #define PA_LOG2E 1.44269504088896340736f
+// The largest probability of a row counts as 2^14 on its way to fp16: one 2^-28 of it is still a normal number and keeps its 11 bits,
+// where relative to 1 those below 2^-14 lose bits and those below 2^-25 are no numbers any more, which adds up where a long row has one
+// key far above all others (17.5 nats above 6000 of them, f32: the others' share was gone).  The running maximum of a row is held
+// 14 lower throughout, so that its sum and its outputs grow alike.
+#define PA_TOP 14.f
 
 // Rows of a tile of many rows, and keys of a block of theirs, by what the registers and two workgroups' LDS hold.  Entries of up to 64
 // rows have one tile of 16 rows to a wave instead of two and take 64 keys whatever their type.
@@ -63,7 +68,7 @@ struct PaParams {
     uint32_t tile_many_log, keys_many_log, keys_64_more;
     PaCosts cost;
     struct PaLeft* entries;  // workspace: what the merge needs of every entry
-    float2* ml;        // maximum (log2 units) and sum of every part's rows
+    float2* ml;        // maximum (log2 units, PA_TOP lower) and sum of every part's rows
     float* o;          // [rows of parts][hd]
 };
 
@@ -408,8 +413,10 @@ __device__ __forceinline__ void pa_store4(void* out, uint32_t dtype, size_t at, 
 // larger one, or none, as 2^70.  Sums of probabilities relative to both ends still meet in fp32 (2^40 times 2^-110).  fp16
 // probabilities that overflow for a scale above that make outputs that are not finite, and such a row is done again.
 __device__ __forceinline__ float pa_exponent(float scale) { return (float)((int)(min(max(__float_as_uint(scale) & 0x7FFFFFFFu, 87u << 23), 197u << 23) >> 23) - 127); }
-// Natural logarithm of the sum from its maximum in log2 units.
-__device__ __forceinline__ float pa_lse(float m, float l) { return l > 0.f ? (m + log2f(l)) * 0.693147180559945309417f : l == 0.f ? -INFINITY : NAN; }
+// Natural logarithm of the sum from its maximum in log2 units (PA_TOP off both: the logarithm of a sum near 1 has more bits).
+__device__ __forceinline__ float pa_lse(float m, float l) {
+    return l > 0.f ? (m + PA_TOP + log2f(l * 6.103515625e-05f)) * 0.693147180559945309417f : l == 0.f ? -INFINITY : NAN;
+}
 
 // ---------------------------------------------------------------------------
 // Few rows: a request's rest, a small group's prefix.  A wave has 16 rows and shares nothing with the others; operands come from
@@ -426,7 +433,7 @@ __device__ __forceinline__ float pa_lse(float m, float l) { return l > 0.f ? (m 
 // numbers; f32 is split into two fp16 terms (TERMS 2), and so are its probabilities.  One-byte rows: codes are exact fp16 numbers;
 // a K row's scale multiplies the score, a V row's the probability in fp32.  The running maximum is then that of
 // score + exponent of the V scale, so that what is rounded to fp16 is relative to the largest contribution whatever the
-// scales are.
+// scales are (to 2^14 .. 2^15 for that one).
 // ---------------------------------------------------------------------------
 template <int HD, int KVM>
 struct PaBlock {
@@ -585,7 +592,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
                 if constexpr (QC) s += pa_exponent(vs[kt][v]);
                 top = fmaxf(top, s);
             }
-        top = max_rows4(top);
+        top = max_rows4(top) - PA_TOP;
         if (__builtin_amdgcn_ballot_w64(top > m)) {
             const float now = fmaxf(top, m), by = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - now);
             m = now;
@@ -949,7 +956,7 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             top[t] = max_rows4(top[t]);
-            if constexpr (!QC) top[t] *= mul[t];
+            top[t] = QC ? top[t] - PA_TOP : fmaf(top[t], mul[t], -PA_TOP);
             more |= top[t] > m[t];
         }
         if (__builtin_amdgcn_ballot_w64(more)) {

@@ -728,3 +728,51 @@ def test_calls_between_torch_operations(backend):
     r = subprocess.run([sys.executable, os.path.join(here, "paged_torch.py")], env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stdout + r.stderr
     assert r.stdout.split("\n")[:2] == ["the default stream ok", "a side stream ok"]
+
+
+# Rows of one kv head: 4 (a wave to 16 rows), 40 (one tile of 16 rows to a wave), 280 (two of them).
+DOMINATED = {"single": [(0, [(6000, 1)]), (3000, [(50, 1), (700, 1)])], "some": [(0, [(4000, 10)])], "chunk": [(0, [(3000, 70)])]}
+
+
+@pytest.mark.parametrize("gap", [12.0, 17.5])
+@pytest.mark.parametrize("name", DOMINATED)
+@pytest.mark.parametrize("dtype,kv", TYPES)
+def test_attention_one_key_over_thousands(backend, dtype, kv, name, gap):
+    """The first key's score lies `gap` above all others': what the thousands have together is not lost beside it.
+
+    Probabilities are rounded relative to 2^14 times the largest, so fp16 numbers below 2^-14 are off by 2^-25 = 2^-39 times the
+    largest (p s) each, and all others by half a step, 2^-11, or 2^-22 for two terms."""
+    a = Attention(DOMINATED[name], **SMALL, dtype=dtype, kv=kv, seed=7, poison=False, scale=1.0)
+    rng, hd = a.rng, a.hd
+    q = rng.uniform(-0.01, 0.01, (a.t, a.nq, hd))
+    q[..., 0] = 1
+    a.q = pm.to_type(q, dtype)
+    shape = a.rows[0].shape
+    first = np.zeros(shape[1:3], bool)
+    for g in range(len(a.prefix)):
+        first[a.tables[a.cu_g[g], 0], 0] = True
+    small = rng.uniform(-0.01, 0.01, shape)
+    small[..., 0] = 0
+    if kv == "f16":
+        small[:, first] = 0
+        small[:, first, 0] = gap
+        a.rows = [small.astype(np.float16), rng.uniform(0.5, 1.5, shape).astype(np.float16)]
+    else:
+        code = {"i8": lambda x: np.round(x * 12700).astype(np.int8), "fp8": lambda x: rng.integers(0x38, 0x40, shape).astype(np.uint8)}[kv](small)
+        code[..., 0] = 0
+        code[:, first] = 0
+        code[:, first, 0] = 127 if kv == "i8" else 0x7e          # (448)
+        full = 127 if kv == "i8" else 448
+        a.rows = [code, (rng.integers(60, 128, shape).astype(np.int8) if kv == "i8" else rng.integers(0x30, 0x40, shape).astype(np.uint8))]
+        a.scales = [np.where(first, gap / full, 0.01 / 128)[None].repeat(shape[0], 0).astype(np.float32),
+                    rng.uniform(0.5, 1.5, shape[:3]).astype(np.float32) / (64 if kv == "i8" else 1)]
+    a.rows[1][:, first, ::2] = 0                                 # (the others alone make up these dimensions)
+    a.make()
+    a.run().expect()
+    out, lse, mag, low = a.want
+    score = (2.0 ** -22 + hd * U) * a.size
+    got, got_lse = pm.from_type(a.dout.get(), dtype), a.dlse.get()
+    assert np.all(np.abs(got_lse - lse) <= score + 2.0 ** -20 + 2.0 ** -22 * np.abs(lse))
+    p_err = (2.0 ** -11 if dtype != "float32" else 2.0 ** -22) + 2 * score[..., None] + int(a.lens.max()) ** 0.5 * 8 * U + 2.0 ** -20
+    limit = p_err * mag + 2.0 ** -39 * low + HALF_STEP[dtype] * np.abs(out) + (2.0 ** -25 if dtype == "float16" else 0)
+    assert np.max(np.abs(got - out) / limit) <= 1
