@@ -839,7 +839,8 @@ __device__ __forceinline__ void pa_many_rows(const PaParams& p, const PaItem& it
         }
         top = max_rows4(top);
         const int ex = top > 0.f && top < INFINITY ? __builtin_amdgcn_frexp_expf(top) : 0;
-        mul[t] = __builtin_amdgcn_ldexpf(p.scale_log2, ex);
+        // (never 0, which would make the -infinity of a key that is not seen no number: this form multiplies after it has masked)
+        mul[t] = fmaxf(__builtin_amdgcn_ldexpf(p.scale_log2, ex), 1.401298464e-45f);
 #pragma unroll
         for (int s = 0; s < KS; s++)
 #pragma unroll

@@ -776,3 +776,16 @@ def test_attention_one_key_over_thousands(backend, dtype, kv, name, gap):
     p_err = (2.0 ** -11 if dtype != "float32" else 2.0 ** -22) + 2 * score[..., None] + int(a.lens.max()) ** 0.5 * 8 * U + 2.0 ** -20
     limit = p_err * mag + 2.0 ** -39 * low + HALF_STEP[dtype] * np.abs(out) + (2.0 ** -25 if dtype == "float16" else 0)
     assert np.max(np.abs(got - out) / limit) <= 1
+
+
+@pytest.mark.parametrize("how", ["scale", "queries"])
+@pytest.mark.parametrize("dtype,kv", TYPES)
+def test_attention_scores_too_small_for_numbers(backend, dtype, kv, how):
+    """scale times a query's largest value lies below all fp32 numbers: every key that is seen counts the same."""
+    if how == "queries" and dtype == "float16":
+        pytest.skip("a float16 query's smallest value times the scale is a number")
+    a = Attention(MIXED + [(0, [(30, 12)])], **SMALL, dtype=dtype, kv=kv, seed=4, scale=1e-45 if how == "scale" else 2.0 ** -24)
+    a.q = pm.to_type(pm.from_type(a.q, dtype) * (2.0 ** -12 if how == "scale" else 2.0 ** -131), dtype)
+    a.make()
+    a.run().expect().check()
+    assert np.isfinite(a.dlse.get()).all()
