@@ -4,6 +4,7 @@
 #include <cmath>
 
 #include "paged_kernels.h"
+#include "row_overlap.h"
 #include "runtime_internal.h"
 
 using namespace oxb;
@@ -24,6 +25,11 @@ struct OnDevice {
 
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 int bad(const char* what) { return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: %s", what); }
+
+RowSpan row_span(const void* p, uint32_t n, uint64_t wide, uint32_t stride, uint32_t dtype) {
+    const uint64_t size = dtype == OXB_DTYPE_F32 ? 4 : 2;
+    return {(uint64_t)(uintptr_t)p, n, wide * size, stride * size};
+}
 
 int check_page_size(uint32_t page_size, uint32_t n_pages) {
     if (page_size != 16 && page_size != 32 && page_size != 64 && page_size != 128)
@@ -106,6 +112,10 @@ int oxb_hip_paged_rows_dev(const oxb_paged_rows* a) {
     if (!a->d_cos != !a->d_sin || (a->d_cos && (!a->d_positions || a->n_angles == 0))) return bad("RoPE needs cos, sin, positions and a number of angles");
     if (!aligned(a->d_cos, 16) || !aligned(a->d_sin, 16) || !aligned(a->d_q_norm, 16) || !aligned(a->d_k_norm, 16)) return bad("norm vectors or angles are not 16-byte aligned");
     if (int rc = ensure_init()) return rc;
+    const bool in_place = a->d_q_out == a->d_qkv && a->q_dtype == a->qkv_dtype && (a->q_stride == a->qkv_stride || a->n_rows == 1);
+    if (a->d_q_out && !in_place &&
+        rows_overlap(row_span(a->d_qkv, a->n_rows, wide, a->qkv_stride, a->qkv_dtype), row_span(a->d_q_out, a->n_rows, (uint64_t)a->nq * a->pool.hd, a->q_stride, a->q_dtype)))
+        return bad("rows of q_out overlap rows of qkv (it may be qkv itself, with the same type and stride)");
     OnDevice on;
     const hipError_t e = oxb_launch_paged_rows(*a, g_rt.stream);
     return e == hipSuccess ? OXB_HIP_OK : hip_fail(e, "paged rows");
@@ -137,6 +147,8 @@ int oxb_hip_paged_attention_dev(const oxb_paged_attention* a) {
     if (!a->d_workspace || !aligned(a->d_workspace, 256) || a->workspace_bytes < need)
         return fail(OXB_HIP_INVALID_ARGUMENT, "invalid argument: workspace of %zu bytes (%zu needed, 256-byte aligned)", a->d_workspace ? a->workspace_bytes : (size_t)0, need);
     if (int rc = ensure_init()) return rc;
+    if (rows_overlap(row_span(a->d_q, a->n_tokens, wide, a->q_stride, a->dtype), row_span(a->d_out, a->n_tokens, wide, a->out_stride, a->dtype)))
+        return bad("rows of out overlap rows of q, which are still read while rows of out are written");
     OnDevice on;
     const hipError_t e = oxb_launch_paged_attention(*a, g_rt.stream);
     return e == hipSuccess ? OXB_HIP_OK : hip_fail(e, "paged attention");

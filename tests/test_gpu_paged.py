@@ -789,3 +789,28 @@ def test_attention_scores_too_small_for_numbers(backend, dtype, kv, how):
     a.make()
     a.run().expect().check()
     assert np.isfinite(a.dlse.get()).all()
+
+
+def test_rows_that_overlap_are_refused(backend):
+    """Through the C entries too, which see addresses alone; rows that lie side by side in one buffer are taken."""
+    a = Attention(MIXED, **SMALL, dtype="float16", kv="f16", seed=5)
+    t, wide, hd = a.t, a.nq * a.hd, a.hd
+    both = DevArray(pm.to_type(np.concatenate([pm.from_type(a.q, "float16").reshape(t, -1), np.full((t, wide + 64), 9.0)], 1), "float16"), "float16")
+    at = lambda first, stride=2 * wide + 64: both.view(first, (t, a.nq, hd), (stride, hd, 1))  # noqa: E731
+    for out in (at(wide - 8), at(8), at(2 * wide + 64), at(16, wide)):
+        with pytest.raises(GpuError, match="overlap"):
+            a.call(at(0), out, workspace=a.ws)
+    a.call(at(0), at(wide), workspace=a.ws)
+    assert np.array_equal(both.get()[:, wide:2 * wide].reshape(t, a.nq, hd), a.run().dout.get())
+    n, nq, nkv = 6, 4, 2
+    full = (nq + 2 * nkv) * hd
+    x = DevArray(np.zeros((n, 2 * full), np.float32))
+    store = paged.RowStore(a.pool, nq=nq, slots=_i32(np.full(n, -1)), positions=_i32(np.zeros(n)))
+    half = DevArray(None, view=(x, 0, (n, nq, hd), (2 * full, hd, 1)))
+    half.dtype = "x.float16"                                     # (the same addresses as another type)
+    qkv = x.view(0, (n, full), (2 * full, 1))
+    for q in (half, x.view(8, (n, nq, hd), (2 * full, hd, 1)), x.view(0, (n, nq, hd), (full, hd, 1)), x.view(full - 8, (n, nq, hd), (2 * full, hd, 1))):
+        with pytest.raises(GpuError, match="overlap"):
+            store(qkv, q)
+    for q in (x.view(0, (n, nq, hd), (2 * full, hd, 1)), x.view(full, (n, nq, hd), (2 * full, hd, 1))):
+        store(qkv, q)

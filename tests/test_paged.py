@@ -203,3 +203,44 @@ def test_the_null_stream_has_a_name_of_its_own():
     assert seen == [None, 1, 0x7f00, None]      # null restores the library's stream, 1 is OXB_HIP_NULL_STREAM
     header = open(os.path.join(ROOT, "include", "oxb_hip.h")).read()
     assert f"#define OXB_HIP_NULL_STREAM ((void*){_lib.NULL_STREAM})" in header
+
+
+def test_row_overlap_against_all_bytes(tmp_path):
+    """The check behind the refusals of overlapping rows, on small spans whose bytes are marked one by one."""
+    cxx = shutil.which("g++")
+    if not cxx:
+        pytest.skip("no C++ compiler")
+    (tmp_path / "overlap.cpp").write_text("""
+#include <cstdio>
+#include <vector>
+#include "row_overlap.h"
+using oxb::RowSpan;
+static bool plain(const RowSpan& a, const RowSpan& b) {
+    std::vector<char> in(400, 0);
+    for (unsigned i = 0; i < a.n; i++) for (unsigned x = 0; x < a.wide; x++) in[a.at + i * a.stride + x] = 1;
+    for (unsigned i = 0; i < b.n; i++) for (unsigned x = 0; x < b.wide; x++) if (in[b.at + i * b.stride + x]) return true;
+    return false;
+}
+int main() {
+    long n = 0, yes = 0;
+    for (unsigned na = 1; na <= 4; na++) for (unsigned nb = 1; nb <= 4; nb++)
+    for (unsigned wa = 1; wa <= 5; wa += 2) for (unsigned wb = 1; wb <= 5; wb++)
+    for (unsigned sa = wa; sa <= 11; sa += 1) for (unsigned sb = wb; sb <= 11; sb++)
+    for (unsigned at = 0; at <= 100; at += 3) {
+        const RowSpan a = {50, na, wa, sa}, b = {at, nb, wb, sb};
+        const bool want = plain(a, b);
+        if (oxb::rows_overlap(a, b) != want || oxb::rows_overlap(b, a) != want) {
+            printf("%u %u %u %u %u %u %u: %d\\n", na, nb, wa, wb, sa, sb, at, want);
+            return 1;
+        }
+        n++, yes += want;
+    }
+    const RowSpan far = {1ull << 40, 1ull << 30, 64, 1ull << 34}, near = {4096, 8, 64, 64};
+    if (oxb::rows_overlap(far, near) || !oxb::rows_overlap(far, {(1ull << 40) + (5ull << 34) + 63, 3, 64, 1ull << 34})) return 2;
+    printf("%ld %ld\\n", n, yes);
+    return yes > 1000 ? 0 : 3;
+}
+""".replace("\\\\n", "\\n"))
+    subprocess.run([cxx, "-std=c++17", "-O1", "-I", os.path.join(ROOT, "oxibonsai_amd", "csrc"), str(tmp_path / "overlap.cpp"), "-o", str(tmp_path / "overlap")], check=True)
+    r = subprocess.run([str(tmp_path / "overlap")], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout
