@@ -64,6 +64,12 @@ def _at(t, name: str, device):
     return t.data_ptr()
 
 
+def _home(device) -> None:
+    """The library runs on one GPU, this one if it has not started yet; tensors of another are refused."""
+    if device.type == "cuda" and getattr(device, "index", None) is not None:
+        _check(_lib.lib().oxb_hip_init(device.index))
+
+
 def _flat(t, name: str, kind: str, shape, device):
     """Address of a contiguous tensor of this type and shape; None stays None."""
     if t is None:
@@ -92,6 +98,7 @@ class PagePool:
         kind = _kind(k)
         if len(k.shape) != 4 or KV_DTYPES.get(kind) is None:
             raise _bad(f"k is {kind} {tuple(k.shape)}, not float16, int8 or float8_e4m3fn [nkv, n_pages, page_size, hd]")
+        _home(k.device)
         self.device, self.kv_dtype = k.device, KV_DTYPES[kind]
         self.nkv, self.n_pages, self.page_size, self.hd = (int(n) for n in k.shape)
         scales = [None, None]
@@ -119,6 +126,7 @@ class PageAssign(_Bound):
                  n_free_out=None, keep=None):
         if len(tables.shape) != 2 or len(slots.shape) != 1 or len(free_pages.shape) != 1:
             raise _bad("tables is [n_requests, width], slots [n_rows], free_pages [n_pages]")
+        _home(tables.device)
         b, width = (int(n) for n in tables.shape)
         rows, pages, dev = int(slots.shape[0]), int(free_pages.shape[0]), tables.device
         n_free_out = n_free if n_free_out is None else n_free_out

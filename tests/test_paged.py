@@ -244,3 +244,37 @@ int main() {
     subprocess.run([cxx, "-std=c++17", "-O1", "-I", os.path.join(ROOT, "oxibonsai_amd", "csrc"), str(tmp_path / "overlap.cpp"), "-o", str(tmp_path / "overlap")], check=True)
     r = subprocess.run([str(tmp_path / "overlap")], capture_output=True, text=True)
     assert r.returncode == 0, r.stdout
+
+
+def test_binding_refuses_the_tensors_of_another_gpu(monkeypatch):
+    """The library has started on GPU 0: nothing is made for tensors of GPU 1."""
+    real, asked = _lib.lib(), []
+
+    class Started:
+        def __getattr__(self, name):
+            return getattr(real, name)
+
+        def oxb_hip_init(self, index):
+            asked.append(index)
+            return 0 if index == 0 else INVALID
+
+    monkeypatch.setattr(_lib, "lib", Started)
+
+    def on(index, shape, kind):
+        t = Host(shape, kind)
+        t.device.index = index
+        return t
+
+    def pool_on(index):
+        return paged.PagePool(*(on(index, (2, 10, 16, 64), "float16") for _ in "kv"))
+
+    def assign_on(index):
+        i = lambda *shape: on(index, shape, "int32")  # noqa: E731
+        return paged.PageAssign(past=i(3), add=i(3), tables=i(3, 4), free_pages=i(9), n_free=i(1), lens=i(3), cu_tokens=i(4), cu_pages=i(4), slots=i(7),
+                                positions=i(7), status=i(2), page_size=16)
+
+    for make in (pool_on, assign_on):
+        make(0)
+        with pytest.raises(GpuError):
+            make(1)
+    assert asked == [0, 1, 0, 1]
