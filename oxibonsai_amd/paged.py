@@ -64,8 +64,26 @@ def _at(t, name: str, device):
     return t.data_ptr()
 
 
-def _home(device) -> None:
-    """The library runs on one GPU, this one if it has not started yet; tensors of another are refused."""
+_one_runtime = False
+
+
+def _runtimes() -> list[str]:
+    """The HIP runtimes in this process: torch ships one of its own, which a library that is loaded later uses too."""
+    with open("/proc/self/maps") as maps:
+        return sorted({line.split()[-1] for line in maps if "/libamdhip64.so" in line})
+
+
+def _home(t) -> None:
+    """The library runs on one GPU, this one if it has not started yet; tensors of another are refused, and so are those of a torch that
+    brought a second runtime, whose streams and graphs are none to the library."""
+    global _one_runtime
+    device = t.device
+    if not _one_runtime and type(t).__module__.partition(".")[0] == "torch":
+        _lib.lib()
+        found = _runtimes()
+        if len(found) > 1:
+            raise _bad(f"two HIP runtimes are loaded ({', '.join(found)}): import torch before the library is")
+        _one_runtime = True
     if device.type == "cuda" and getattr(device, "index", None) is not None:
         _check(_lib.lib().oxb_hip_init(device.index))
 
@@ -98,7 +116,7 @@ class PagePool:
         kind = _kind(k)
         if len(k.shape) != 4 or KV_DTYPES.get(kind) is None:
             raise _bad(f"k is {kind} {tuple(k.shape)}, not float16, int8 or float8_e4m3fn [nkv, n_pages, page_size, hd]")
-        _home(k.device)
+        _home(k)
         self.device, self.kv_dtype = k.device, KV_DTYPES[kind]
         self.nkv, self.n_pages, self.page_size, self.hd = (int(n) for n in k.shape)
         scales = [None, None]
@@ -126,7 +144,7 @@ class PageAssign(_Bound):
                  n_free_out=None, keep=None):
         if len(tables.shape) != 2 or len(slots.shape) != 1 or len(free_pages.shape) != 1:
             raise _bad("tables is [n_requests, width], slots [n_rows], free_pages [n_pages]")
-        _home(tables.device)
+        _home(tables)
         b, width = (int(n) for n in tables.shape)
         rows, pages, dev = int(slots.shape[0]), int(free_pages.shape[0]), tables.device
         n_free_out = n_free if n_free_out is None else n_free_out

@@ -4,6 +4,7 @@ import ctypes as C
 import os
 import shutil
 import subprocess
+import sys
 from types import SimpleNamespace
 
 import numpy as np
@@ -278,3 +279,13 @@ def test_binding_refuses_the_tensors_of_another_gpu(monkeypatch):
         with pytest.raises(GpuError):
             make(1)
     assert asked == [0, 1, 0, 1]
+
+
+@pytest.mark.parametrize("first", ["torch", "library"])
+def test_torch_after_the_library_is_refused(first):
+    """Loaded the other way round, torch brings a HIP runtime that knows nothing of the library's streams."""
+    load = {"torch": "import torch", "library": "from oxibonsai_amd import _lib; _lib.lib()"}
+    program = "\n".join([load[first], *load.values(), "from oxibonsai_amd import paged", "k = torch.zeros((1, 1, 16, 32), dtype=torch.float16)", "paged.PagePool(k, k)"])
+    r = subprocess.run([sys.executable, "-c", program], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    wanted = "not on a GPU" if first == "torch" else "two HIP runtimes"     # (here on the CPU both end with an error)
+    assert r.returncode != 0 and wanted in r.stderr, r.stderr
