@@ -326,3 +326,29 @@ def test_batched_gemv_captured_cold_into_a_callers_graph(backend):
         d_x.free()
         d_y.free()
         backend.free_weights(h)
+
+
+def test_calls_on_the_null_stream(backend):
+    """HIP's null stream, whose handle is 0, by its own name: products and the model's step give the bits of the library's stream."""
+    cfg = dict(fmt=Q1, n_layers=2, h=256, inter=512, nq=4, nkv=2, hd=64, vocab=96, max_seq=32, eps=1e-6, rope_theta=1e6)
+    w = synth.make_model(cfg, 912)
+    rows = [synth.embedding_rows(913, [i], cfg["h"])[0] * 50.0 for i in range(5)]
+    a, x = synth.make_blocks(TQ2, 914, 96, 512), synth.normal_f32(915, 40 * 512).reshape(40, 512)
+    h = backend.upload_weights_ternary(a, 96, 512)
+
+    def run():
+        model = HipModel(backend, cfg, w, batch=1)
+        try:
+            got = [model.forward(r, i)[0][0].copy() for i, r in enumerate(rows)]
+            return got + [model.uses_graph(), backend.gemv_cached_batch(h, x[:3], 96, 512), backend.gemm_tq2_g128(a, x, 40, 96, 512)]
+        finally:
+            model.close()
+
+    want = run()
+    backend.set_stream(0)
+    try:
+        got = run()
+    finally:
+        backend.set_stream(None)
+        backend.free_weights(h)
+    assert all(np.array_equal(a, b) for a, b in zip(got, want)) and got[5] is True
