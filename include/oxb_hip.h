@@ -283,10 +283,10 @@ int  oxb_hip_paged_assign_dev(const oxb_page_assign* a);
  * cos, sin [n_angles][hd / 2] of the row's position (both NULL: not rotated), as fused_qk_norm_rope does
  * (KG/cuda_attn_kernels.rs:160-226); q goes to q_out [n_rows][nq][hd] (NULL: q is not looked at), k and v to slot slots[t] of the
  * pool: rounded to fp16, or as codes round(x / scale) of oxb_hip_kv_quantize_rows' types with scale = max|x| times the fp32
- * reciprocal of the largest code, at least 2^-23 (the quantiser's own scale is the quotient: an ulp apart at most).  A row whose position is negative (or has no angles, where it
- * is rotated) is left out; one whose slot is negative or behind the pool leaves no k and v.  positions may be NULL where nothing
+ * reciprocal of the largest code, at least 2^-23 (the quantiser's own scale is the quotient: an ulp apart at most).  A row whose
+ * position is negative (or has no angles, where it is rotated) is left out; one whose slot is negative or behind the pool leaves no k and v.  positions may be NULL where nothing
  * is rotated: no row is left out then.  Two rows with one slot leave a mixture there.  Strides are in elements, multiples of 8;
- * qkv and q_out 16-byte aligned.  q_out may be qkv, where type and stride are the same; other rows that overlap are
+ * qkv and q_out 16-byte aligned; n_rows at least 1.  q_out may be qkv, where type and stride are the same; other rows that overlap are
  * refused. */
 typedef struct {
     uint32_t n_rows, nq;
@@ -311,7 +311,8 @@ int  oxb_hip_paged_rows_dev(const oxb_paged_rows* a);
  * the ones that the group's FIRST request's table names, and are read once for all the group's queries.  n_groups 0: nothing is
  * shared; else cu_groups[0] = 0 and cu_groups[n_groups] = n_requests.
  * q, out: one type (f32: fp32-level accuracy, scores and probabilities as two fp16 terms; f16, bf16: probabilities are
- * rounded to fp16).  Strides in elements, multiples of 8; 16-byte aligned; rows of out that overlap rows of q are refused.  scale 0 stands for 1 / sqrt(hd).  n_requests 1 .. 4096.
+ * rounded to fp16).  Strides in elements, multiples of 8; 16-byte aligned; rows of out that overlap rows of q are refused.
+ * scale 0 stands for 1 / sqrt(hd).  n_requests 1 .. 4096, n_tokens at least 1.
  * A value that is infinite or no number reaches the queries that see its key and no others; such queries are slow (a key at a
  * time).  Scales of value rows keep this accuracy from 2^-40 on; smaller ones lose what lies below 2^-79.
  * Queries times table_width are limited: n_tokens nq / 16 + (n_requests + n_groups) nkv tiles of rows, twice that with groups, times

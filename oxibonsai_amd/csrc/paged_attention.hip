@@ -17,9 +17,12 @@
 // each other.  The first workgroup of a CU takes from the first half, where the prefixes are, which are bound by the matrix
 // cores, the second one from the second half, where the rests are, which are bound by memory.
 //
-// Calls, 32 q heads on 8 kv heads of 128: 62 requests of 700 keys behind 4100 shared ones, fp16 rows, 40.5 us (107 MB, 22.7 us
-// at a copy's rate; 33 in the first launch = 3.2 TB/s), 256 of 900 behind 16 000 162 us (542 MB), 14 chunks of 300 behind 3500
-// 165 us (89 GFLOP, 0.6 PFLOP/s in the first launch), 90 requests of 400 behind 2000, INT8 rows, f32, 40.3 us.
+// Calls, 32 q heads on 8 kv heads of 128: 62 requests of up to 700 keys (350 on average) behind 4100 shared ones, fp16 rows, 41 us
+// (107 MB, 22.7 us at a copy's rate; 34 in the first launch = 3.1 TB/s), 256 of up to 900 (450) behind 16 000 160 us (542 MB), 14
+// chunks of up to 300 queries (105) behind 3500 keys 158 to 167 us (89 GFLOP, 0.5 to 0.6 PFLOP/s in the first launch), 90 requests of
+// up to 400 (200) behind 2000, INT8 rows, f32, 40.6 us.
+// Every form of the first kernel keeps 65 to 102 scalar registers in lanes of a vector register (the plan, the parameters); f32 on
+// one-byte rows of 128 has 15 (INT8) and 17 (FP8) vector registers too many, 64 and 72 bytes of scratch a lane.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -37,7 +40,7 @@ typedef uint32_t v2w __attribute__((ext_vector_type(2)));
 #define PA_TILE_FEW_LOG 4u
 #define PA_KEYS_FEW_LOG 5u // keys that such a wave takes at a time: 32
 #define PA_RUNS 256u       // runs of entries, one to a thread
-#define PA_STAGED 240u     // requests up to which a workgroup copies the lengths to LDS first
+#define PA_STAGED 240u     // requests up to which a workgroup copies the lengths to LDS first (81 776 bytes, two workgroups have 81 920 each)
 #define PA_OWN 96u         // rows of a group's requests, on average, from which on they do not share their prefix' walk (48, 1600: within 1 %)
 #define PA_MERGE_WIDE 512u  // rows of outputs up to which the merge reads a row's parts in eight groups of lanes (100: 9 questions about 60 000 keys 59.5 us instead of 54)
 #define PA_LOG2E 1.44269504088896340736f
@@ -688,7 +691,7 @@ __device__ __forceinline__ void pa_few_rows(const PaParams& p, const PaItem& it)
 // row number, so that neither the reads of K (16 rows, one piece) nor the transposing reads of V meet in a bank.
 //
 // The same products and softmax as above; V's operand comes from the transposing reads.  Bound by issue: matrix instructions (0.27
-// of the SIMDs' time in 14 chunks of 300 queries behind 3500 keys), LDS reads, of which two tiles share each, and the VALU's softmax;
+// of the SIMDs' time in 14 chunks of up to 300 queries behind 3500 keys), LDS reads, of which two tiles share each, and the VALU's softmax;
 // 0.30 of the waves' time waits for its turn to issue.
 // ---------------------------------------------------------------------------
 // K and V of two blocks: arrays of their own, so that the compiler sees that a read of one need not wait for what is on its way
@@ -1083,8 +1086,9 @@ __global__ __launch_bounds__(256, HD == 256 ? 1 : 2) void paged_attention_kernel
 // ---------------------------------------------------------------------------
 // A row over again, key by key and only the keys that it sees, by HD / 4 lanes.  The products of a block that only some of its rows see
 // multiply the values of a key that a row does not see by 0, which is no number where that value, or its row's scale, is infinite or
-// none itself: such rows, a finite sum of probabilities beside an output that is not finite, come here.  Slow (a key at a time)
-// and rare; with infinities that the row does see the answer is the same as before.
+// none itself: such rows, a finite sum of probabilities beside an output that is not finite, come here.  Slow (a key at a time, and
+// rows that do see such a value come too: one in a shared prefix sends all of the group's here) and rare; with infinities that the
+// row does see the answer is the same as before.
 // ---------------------------------------------------------------------------
 template <int HD>
 __device__ __forceinline__ void pa_row_again(const PaParams& p, uint32_t r, uint32_t t, uint32_t h, uint32_t c, float o[4]) {
@@ -1145,8 +1149,8 @@ __device__ __forceinline__ void pa_row_again(const PaParams& p, uint32_t r, uint
 // ---------------------------------------------------------------------------
 // The parts of every row brought to a common maximum and added in order: the prefix' parts, then the rest's.  HD / 4 lanes to a row and
 // every GROUPS-th part, whose sums meet in LDS: eight where the rows are few and may have been cut into very many parts, whose reads
-// would follow each other, else one.  Latency bound: 5.5 us for 80 rows, 7 for 1984, 24 for 134 000 of 14 chunks, most
-// of whose tokens have rows in two shares (a look at all of a token's rows first: 27).
+// would follow each other, else one.  Latency bound for few rows: 6 us for 80, 7.5 for 1984.  The 47 008 of 14 chunks, most of which
+// lie in two shares, take 23 to 26: about 48 MB of parts at 2 TB/s (a look at all of a token's rows first: 27).
 // ---------------------------------------------------------------------------
 template <int HD, int GROUPS>
 __global__ __launch_bounds__(256) void paged_merge_kernel(PaParams p) {
